@@ -68,6 +68,16 @@ class AugmentParams(ctypes.Structure):
                 ("crop_b", c_int), ("out_h", c_int), ("out_w", c_int)]
 
 
+class Linear(ctypes.Structure):
+    """psfm_linear (include/psfm_linear.h)."""
+    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("ldr", ctypes.c_int64), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("p", ctypes.c_double),
+                ("mask_rows", ctypes.c_int64), ("rng", c_void_p)]
+
+
+# PSFM_DTYPE_* (include/psfm_dropout.h)
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
 _lib = None
 REPO_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -183,6 +193,17 @@ def lib():
         "psfm_train_augment": ([ctypes.POINTER(AugmentParams), V, V, V, V, V, V, V], c_int),
         "psfm_gather_frames": ([c_int, V, V, V, V, c_int, c_int, c_int, V, V, V], c_int),
         "psfm_augment_last_error": ([], ctypes.c_char_p),
+        # include/psfm_dropout.h
+        "psfm_dropout": ([V, ctypes.c_int64, V, ctypes.c_int64, c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                          ctypes.c_double, V, V, V], c_int),
+        "psfm_rng_next": ([V, V, V], c_int),
+        "psfm_dropout_last_error": ([], ctypes.c_char_p),
+        # include/psfm_linear.h
+        "psfm_linear_fwd_ws_bytes": ([ctypes.POINTER(Linear)], ctypes.c_int64),
+        "psfm_linear_fwd": ([ctypes.POINTER(Linear), V, V, V, V, V, V, V, V], c_int),
+        "psfm_linear_bwd_ws_bytes": ([ctypes.POINTER(Linear), c_int, c_int, c_int], ctypes.c_int64),
+        "psfm_linear_bwd": ([ctypes.POINTER(Linear), V, V, V, V, V, V, V, V, V], c_int),
+        "psfm_linear_last_error": ([], ctypes.c_char_p),
         # include/psfm_pose.h
         "psfm_pose_from_vec_fwd": ([V, c_int, c_int, V, V], c_int),
         "psfm_pose_from_vec_bwd": ([V, c_int, c_int, V, V, V], c_int),
@@ -222,6 +243,9 @@ EXPORTED = ("psfm_workspace_floats", "psfm_photometric_clip_stats", "psfm_photom
             "psfm_pc_compose_bwd", "psfm_pc_fwd", "psfm_pc_bwd", "psfm_pc_last_error",
             "psfm_augment_plan", "psfm_augment_ws_bytes", "psfm_train_augment", "psfm_gather_frames",
             "psfm_augment_last_error",
+            "psfm_dropout", "psfm_rng_next", "psfm_dropout_last_error",
+            "psfm_linear_fwd_ws_bytes", "psfm_linear_fwd", "psfm_linear_bwd_ws_bytes", "psfm_linear_bwd",
+            "psfm_linear_last_error",
             "psfm_pose_from_vec_fwd", "psfm_pose_from_vec_bwd", "psfm_pinhole_cam_records", "psfm_pose_last_error",
             "psfm_knob_count", "psfm_knob_name", "psfm_knob_default", "psfm_knob_value", "psfm_knob_set",
             "psfm_knob_rejected")
@@ -266,6 +290,10 @@ def check(rc, what):
             err = lib().psfm_metrics_last_error
         elif what.startswith(("psfm_augment", "psfm_train_augment", "psfm_gather_frames")):
             err = lib().psfm_augment_last_error
+        elif what.startswith(("psfm_dropout", "psfm_rng_next")):
+            err = lib().psfm_dropout_last_error
+        elif what.startswith("psfm_linear"):
+            err = lib().psfm_linear_last_error
         elif what.startswith(("psfm_pose_from_vec", "psfm_pinhole_cam_records")):
             err = lib().psfm_pose_last_error
         elif what.startswith("psfm_p3d"):
@@ -330,6 +358,10 @@ def _install_capture_hooks():
 # then segfaults in capture_end — by the time the op's own backward runs, the autograd engine has
 # already recorded that wait, so the refusal has to come before the capture exists.
 _EAGER_CTX = weakref.WeakSet()
+# Contexts whose backward has run, whose graph still lives (its output is held) and whose forward ran on the
+# default stream: the graph keeps its leaves' gradient accumulators, which are bound to that stream, and a
+# captured backward of the same leaves would accumulate there; the default stream cannot join a capture.
+_EAGER_DONE = weakref.WeakSet()
 
 
 def note_forward(ctx):
@@ -353,22 +385,32 @@ def _refuse_stray_backward(cap_stream):
             "backpropagated; a backward captured for them would run on their forward's stream, outside the "
             "capture (HIP segfaults in capture_end).  Run the backward (or free the graph) first, or run the "
             "forward inside the same capture, as DDPTrainer.capture does")
+    with _CAPTURE_LOCK:
+        held = sorted({type(c).__name__ for c in list(_EAGER_DONE)})
+    if held:
+        raise RuntimeError(
+            f"psfm: refusing to begin a HIP-graph capture while outputs of {', '.join(held)} from an eager step on the "
+            "default stream are held: their graphs keep the leaves' gradient accumulators on that stream, which a "
+            "captured backward cannot use.  Free those outputs first (or run the eager steps on a side stream)")
 
 
 _install_capture_hooks()
 
 
-def capture_guard(ctx=None):
+def capture_guard(ctx=None, leaves=False):
     """Raise before anything is allocated or launched when this thread is not capturing while a
     HIP-graph capture is in progress — called first thing in every HIP backward: PyTorch-ROCm runs a
     node's backward on its forward's stream, so a backward captured for a forward that ran outside
     the capture would otherwise allocate and launch on a stream the capture does not own, and HIP
     segfaults in capture_end.  `ctx` (the op's autograd context) leaves
     the set of pending eager forwards (note_forward) here.  The capture_begin hook refuses such a
-    capture before it starts; this check is the last line for anything it cannot see."""
+    capture before it starts; this check is the last line for anything it cannot see.  `leaves`: the
+    context goes on being watched for the leaves that its graph holds (_EAGER_DONE)."""
     if ctx is not None:
         with _CAPTURE_LOCK:
             _EAGER_CTX.discard(ctx)
+            if leaves and getattr(ctx, "_psfm_stream", None) == 0:
+                _EAGER_DONE.add(ctx)
     if _ACTIVE_CAPTURES and not torch.cuda.is_current_stream_capturing():
         # Refuse — but first join this stream into the capture and straight back (an empty fork), so
         # the capture is still well formed when the error unwinds through torch.cuda.graph: the

@@ -1,0 +1,9 @@
+// psfm_linear_bf16.hip — the pointwise product's kernels for __bf16 (psfm_linear_kernels.h).
+#include "psfm_linear_kernels.h"
+
+namespace psfm {
+const LinearOps& linear_ops_bf16() {
+    static const LinearOps ops = {gemm_of<__bf16>, join_of<__bf16>, dz_of<__bf16>, colsum_of<__bf16>};
+    return ops;
+}
+}  // namespace psfm

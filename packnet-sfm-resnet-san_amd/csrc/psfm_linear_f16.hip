@@ -1,0 +1,9 @@
+// psfm_linear_f16.hip — the pointwise product's kernels for _Float16 (psfm_linear_kernels.h).
+#include "psfm_linear_kernels.h"
+
+namespace psfm {
+const LinearOps& linear_ops_f16() {
+    static const LinearOps ops = {gemm_of<_Float16>, join_of<_Float16>, dz_of<_Float16>, colsum_of<_Float16>};
+    return ops;
+}
+}  // namespace psfm

@@ -1,0 +1,9 @@
+// psfm_linear_f32.hip — the pointwise product's kernels for float (psfm_linear_kernels.h).
+#include "psfm_linear_kernels.h"
+
+namespace psfm {
+const LinearOps& linear_ops_f32() {
+    static const LinearOps ops = {gemm_of<float>, join_of<float>, dz_of<float>, colsum_of<float>};
+    return ops;
+}
+}  // namespace psfm

@@ -1,0 +1,441 @@
+// psfm_linear_kernels.h — the pointwise product's kernels, one instance set per type (gfx950).
+//
+//   k_gemm    one output tile [BI, BJ] per workgroup on the matrix cores.  LDS holds two stages of 128 bytes
+//             of reduction per output row and column (64 values of 16 bits, 32 of 32): while one is multiplied
+//             the next one's global loads are in flight.  The product is taken as D = Q P^T, so that a
+//             lane's four results are four consecutive columns of one output row: one mask block, one
+//             vector store.
+//   k_join    sums split products in the order of their splits, then the same epilogue.
+//   k_dz      dz = drop(dy) act'(z) and its column sums, one pass.
+//   k_colsum  the column sums' partial rows.
+#pragma once
+#include "psfm_linear.h"
+
+namespace psfm {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+constexpr int CHUNK = 16 / (int)sizeof(T);   // values of one 16-byte chunk
+
+// ---- activations, in fp32 ---------------------------------------------------------------------
+__device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float act_of(int act, float z) {
+    switch (act) {
+        case PSFM_ACT_RELU: return z < 0.0f ? 0.0f : z;     // NaN stays
+        case PSFM_ACT_SIGMOID: return sigmoidf(z);
+        case PSFM_ACT_ELU: return z > 0.0f ? z : expm1f(z);
+        case PSFM_ACT_SILU: return z / (1.0f + __expf(-z));
+        case PSFM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float slope_of(int act, float z) {
+    switch (act) {
+        case PSFM_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        case PSFM_ACT_SIGMOID: {
+            const float s = sigmoidf(z);
+            return s * (1.0f - s);
+        }
+        case PSFM_ACT_ELU: return z > 0.0f ? 1.0f : __expf(z);
+        case PSFM_ACT_SILU: {
+            const float s = sigmoidf(z);
+            return s * (1.0f + z * (1.0f - s));
+        }
+        case PSFM_ACT_GELU:
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+        default: return 1.0f;
+    }
+}
+
+// ---- chunks of up to 16 bytes at any alignment that the type has -------------------------------
+template <typename T>
+__device__ __forceinline__ u4v load_chunk(const T* p) {
+    return *reinterpret_cast<const u4v*>(p);
+}
+template <typename T>
+__device__ __forceinline__ u4v load_part(const T* p, int n) {   // the first n values, zeros behind
+    union {
+        u4v v;
+        T t[CHUNK<T>];
+    } u;
+    u.v = u4v{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < CHUNK<T>; ++k)
+        if (k < n) u.t[k] = p[k];
+    return u.v;
+}
+// n in 0 .. CHUNK values at p; VEC: n is 0 or CHUNK and p is 16-byte aligned
+template <typename T, bool VEC>
+__device__ __forceinline__ u4v load_n(const T* p, int n) {
+    if (n >= CHUNK<T>) {
+        if (VEC) return load_chunk(p);
+        u4v v;
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    }
+    return VEC ? u4v{0, 0, 0, 0} : load_part(p, n);
+}
+
+// ---- the epilogue of four consecutive columns j .. j + 3 (n of them exist) of row i ------------
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float v[4], int n, bool whole) {
+    if (whole) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<T4*>(p) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < n) p[k] = (T)v[k];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float v[4], int n, bool whole) {
+    if (whole) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T4 t = *reinterpret_cast<const T4*>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (float)t[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = k < n ? (float)p[k] : 0.0f;
+    }
+}
+
+// mrow: row i's mask row
+template <typename T, bool FULL>
+__device__ __forceinline__ void epilogue4(const LinearEpi& e, const PhiloxKey& key, int64_t J, int64_t i, int64_t mrow,
+                                          int64_t j, float v[4]) {
+    const int n = J - j < 4 ? (int)(J - j) : 4;
+    const bool whole = e.whole;
+    const int64_t at = i * J + j;
+    if (!FULL) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= e.alpha;
+        store4((T*)e.out + at, v, n, whole);
+        return;
+    }
+    if (e.bias) {
+        float b[4];
+        load4((const T*)e.bias + j, b, n, whole);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += b[k];
+    }
+    if (e.z) store4((T*)e.z + at, v, n, whole);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = act_of(e.act, v[k]);
+    if (e.drop.rng) {
+        uint32_t w[4];
+        philox4(key, mask_block(mrow, J, j), w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = w[k] <= e.drop.last ? 0.0f : v[k] * e.drop.scale;
+    }
+    if (e.res) {
+        float r[4];
+        load4((const T*)e.res + i * e.ldr + j, r, n, e.whole_res);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += r[k];
+    }
+    store4((T*)e.out + at, v, n, whole);
+}
+
+// ---- LDS images ----------------------------------------------------------------------------
+// Straight operand: one 128-byte row of reduction per output row; its eight 16-byte chunks are XORed by the
+// row so that 16 lanes reading the same chunk of 16 rows hit 16 bank quads.  Turned operand: one row per
+// reduction index, chunks XORed so that the transposing reads (16 bits: 4 rows x 32 bytes a 16-lane group;
+// 32 bits: 64 bytes a group, 4 groups 4 rows apart) spread over the banks.
+__device__ __forceinline__ int swz_straight(int row) { return (row >> 1) & 7; }
+template <typename T, int B>
+__device__ __forceinline__ int swz_turned(int row) {
+    if (sizeof(T) == 4) return ((row >> 2) & 3) << 2;
+    if (B == 64) return (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) << 1;
+    return ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
+}
+
+// Thread t's share of a stage, NC chunks: global -> registers, registers -> LDS.
+template <typename T, int B, int NTH, bool TURNED, bool VEC>
+struct Stager {
+    static constexpr int NC = B * 8 / NTH, V = CHUNK<T>, CPR = B * (int)sizeof(T) / 16;
+    u4v r[NC];
+
+    // rows b0 .. of extent `ext`, reduction r0 .. rend
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t b0, int64_t ext, int64_t r0, int64_t rend) {
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const int c = q * NTH + threadIdx.x;
+            const int64_t row = TURNED ? r0 + c / CPR : b0 + c / 8;
+            const int64_t col = TURNED ? b0 + (int64_t)(c % CPR) * V : r0 + (c % 8) * V;
+            const int64_t left = row < (TURNED ? rend : ext) ? (TURNED ? ext : rend) - col : 0;
+            r[q] = load_n<T, VEC>(base + (left > 0 ? row * ld + col : 0), left >= V ? V : left > 0 ? (int)left : 0);
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* lds) const {
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const int c = q * NTH + threadIdx.x;
+            const int row = TURNED ? c / CPR : c / 8, ch = TURNED ? c % CPR : c % 8;
+            const int x = TURNED ? swz_turned<T, B>(row) : swz_straight(row);
+            *reinterpret_cast<u4v*>(lds + row * (TURNED ? CPR * 16 : 128) + ((ch ^ x) << 4)) = r[q];
+        }
+    }
+};
+
+// One lane's operand of a matrix instruction step (64 bytes of reduction: 32 values of 16 bits, 16 of 32): the 16
+// output rows or columns b .. b + 15, lane l holds row l % 16, reduction chunk l / 16.
+template <typename T, int B, bool TURNED>
+__device__ __forceinline__ u4v fragment(const uint8_t* lds, int b, int ks) {
+    const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
+    if (!TURNED) {
+        const int row = b + n;
+        return *reinterpret_cast<const u4v*>(lds + row * 128 + (((ks * 4 + g) ^ swz_straight(row)) << 4));
+    }
+    constexpr int RB = B * (int)sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+        u4v v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = ks * 16 + 4 * g + i, ch = (b >> 2) + (n >> 2);
+            v[i] = *reinterpret_cast<const uint32_t*>(lds + row * RB + ((ch ^ swz_turned<T, B>(row)) << 4) + 4 * (n & 3));
+        }
+        return v;
+    } else {
+        // a 16-lane group reads 4 rows x 16 values, lane n gets column n of the 4 rows
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const int ch = (b >> 3) + ((n & 3) >> 1), r0 = ks * 32 + 8 * g + (n >> 2), r1 = r0 + 4;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4*)(lds + r0 * RB + ((ch ^ swz_turned<T, B>(r0)) << 4) + 8 * (n & 1)));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4*)(lds + r1 * RB + ((ch ^ swz_turned<T, B>(r1)) << 4) + 8 * (n & 1)));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(u4v, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ f4 mma(u4v a, u4v b, f4 c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)   // the four 16-value steps take the same reduction order of both operands
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, __bf16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+}
+
+// Workgroup id -> tile: the eight XCDs take turns in the id, so each gets a run of consecutive tiles (its L2
+// keeps their operands), and a run walks 8 tile rows before the next tile column.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
+    const uint32_t x = id & 7, k = id >> 3, per = n >> 3, more = n & 7;
+    return x * per + (x < more ? x : more) + k;
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, bool VEC, bool FULL>
+__global__ __launch_bounds__(64 * WI * WJ) void k_gemm(const GemmArgs A) {
+    constexpr int NTH = 64 * WI * WJ, BR = 128 / (int)sizeof(T), SI = BI / WI / 16, SJ = BJ / WJ / 16;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2][(BI + BJ) * 128];
+    const uint32_t tiles = A.ti * A.tj, w = xcd_run(blockIdx.x, gridDim.x), split = w / tiles, t = w - split * tiles;
+    const uint32_t band = t / (8 * A.tj), in = t - band * 8 * A.tj, high = A.ti - band * 8 < 8 ? A.ti - band * 8 : 8;
+    const int64_t i0 = (int64_t)(band * 8 + in % high) * BI, j0 = (int64_t)(in / high) * BJ;
+    const int64_t r0 = split * A.rsplit, rend = r0 + A.rsplit < A.R ? r0 + A.rsplit : A.R;
+    const int nk = (int)((rend - r0 + BR - 1) / BR);
+    const int wave = threadIdx.x >> 6, wi = wave % WI, wj = wave / WI;
+
+    f4 acc[SI][SJ];
+#pragma unroll
+    for (int a = 0; a < SI; ++a)
+#pragma unroll
+        for (int b = 0; b < SJ; ++b) acc[a][b] = f4{0, 0, 0, 0};
+    Stager<T, BI, NTH, PT, VEC> sp;
+    Stager<T, BJ, NTH, QT, VEC> sq;
+    const T* P = (const T*)A.P;
+    const T* Q = (const T*)A.Q;
+    if (nk > 0) {
+        sp.load(P, A.ldp, i0, A.I, r0, rend);
+        sq.load(Q, A.ldq, j0, A.J, r0, rend);
+        sp.store(smem[0]);
+        sq.store(smem[0] + BI * 128);
+    }
+    __syncthreads();
+    for (int k = 0; k < nk; ++k) {
+        const bool more = k + 1 < nk;
+        if (more) {
+            sp.load(P, A.ldp, i0, A.I, r0 + (int64_t)(k + 1) * BR, rend);
+            sq.load(Q, A.ldq, j0, A.J, r0 + (int64_t)(k + 1) * BR, rend);
+        }
+        const uint8_t* lp = smem[k & 1];
+        const uint8_t* lq = lp + BI * 128;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u4v fp[SI], fq[SJ];
+#pragma unroll
+            for (int a = 0; a < SI; ++a) fp[a] = fragment<T, BI, PT>(lp, wi * (BI / WI) + a * 16, ks);
+#pragma unroll
+            for (int b = 0; b < SJ; ++b) fq[b] = fragment<T, BJ, QT>(lq, wj * (BJ / WJ) + b * 16, ks);
+#pragma unroll
+            for (int a = 0; a < SI; ++a)
+#pragma unroll
+                for (int b = 0; b < SJ; ++b) acc[a][b] = mma<T>(fq[b], fp[a], acc[a][b]);
+        }
+        if (more) {   // the stage that the next step reads; its last readers passed the barrier before this step
+            sp.store(smem[(k + 1) & 1]);
+            sq.store(smem[(k + 1) & 1] + BI * 128);
+        }
+        __syncthreads();
+    }
+
+    const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
+    PhiloxKey key{};
+    if (FULL && A.e.drop.rng && A.splits == 1) key = philox_key(A.e.drop.rng);
+#pragma unroll
+    for (int a = 0; a < SI; ++a) {
+        const int64_t i = i0 + wi * (BI / WI) + a * 16 + n;
+        if (i >= A.I) continue;
+        const int64_t mrow = FULL ? mask_row(A.e.drop, i) : 0;
+#pragma unroll
+        for (int b = 0; b < SJ; ++b) {
+            const int64_t j = j0 + wj * (BJ / WJ) + b * 16 + 4 * g;
+            if (j >= A.J) continue;
+            float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+            if (A.splits > 1)
+                store4(A.part + (split * A.I + i) * A.J + j, v, A.J - j < 4 ? (int)(A.J - j) : 4, (A.J & 3) == 0);
+            else
+                epilogue4<T, FULL>(A.e, key, A.J, i, mrow, j, v);
+        }
+    }
+}
+
+// One thread: four columns of one row, summed over the splits in order.
+template <typename T, bool FULL>
+__global__ __launch_bounds__(256) void k_join(const GemmArgs A) {
+    // a split product is small: its 4-column groups are counted in 32 bits
+    const uint32_t cb = (uint32_t)((A.J + 3) >> 2), id = blockIdx.x * 256 + threadIdx.x, row = id / cb;
+    if (row >= A.I) return;
+    const int64_t i = row, j = (int64_t)(id - row * cb) * 4;
+    const int n = A.J - j < 4 ? (int)(A.J - j) : 4;
+    float v[4] = {0, 0, 0, 0};
+    for (int s = 0; s < A.splits; ++s) {
+        float p[4];
+        load4(A.part + (s * A.I + i) * A.J + j, p, n, (A.J & 3) == 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += p[k];
+    }
+    PhiloxKey key{};
+    if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
+    epilogue4<T, FULL>(A.e, key, A.J, i, FULL ? mask_row(A.e.drop, i) : 0, j, v);
+}
+
+// Workgroup (x, y): 4-column groups x * CB .. of rows y * rows ..; 256 / CB rows at a time.
+template <typename T, int CB>
+__global__ __launch_bounds__(DZ_THREADS) void k_dz(const DzArgs A) {
+    constexpr int RP = DZ_THREADS / CB;
+    __shared__ float sums[RP][CB * 4];
+    const int cx = threadIdx.x % CB, ry = threadIdx.x / CB;
+    const int64_t j = ((int64_t)blockIdx.x * CB + cx) * 4;
+    const int n = A.N - j < 4 ? (int)(A.N - j) : 4;
+    const bool whole = A.whole;
+    const int64_t m0 = (int64_t)blockIdx.y * A.rows, m1 = m0 + A.rows < A.M ? m0 + A.rows : A.M;
+    PhiloxKey key{};
+    if (A.drop.rng) key = philox_key(A.drop.rng);
+    float sum[4] = {0, 0, 0, 0};
+    if (n > 0) {
+        for (int64_t m = m0 + ry; m < m1; m += RP) {
+            float d[4], zv[4];
+            load4((const T*)A.dy + m * A.N + j, d, n, whole);
+            if (A.z) load4((const T*)A.z + m * A.N + j, zv, n, whole);
+            if (A.z) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] *= slope_of(A.act, zv[k]);
+            }
+            if (A.drop.rng) {   // last: a dropped value is 0 whatever dy and z hold
+                uint32_t w[4];
+                philox4(key, mask_block(mask_row(A.drop, m), A.N, j), w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = w[k] <= A.drop.last ? 0.0f : d[k];
+            }
+            if (A.dz) store4((T*)A.dz + m * A.N + j, d, n, whole);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] += d[k];
+        }
+    }
+    if (!A.part) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[ry][cx * 4 + k] = sum[k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < CB * 4; c += DZ_THREADS) {
+        const int64_t col = (int64_t)blockIdx.x * CB * 4 + c;
+        if (col >= A.N) continue;
+        float s = 0;
+        for (int r = 0; r < RP; ++r) s += sums[r][c];
+        A.part[blockIdx.y * A.N + col] = s;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_colsum(const float* part, int64_t parts, int64_t N, float alpha, T* db) {
+    __shared__ float sums[4][64];
+    const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+    float s = 0;
+    if (col < N)
+        for (int64_t p = q; p < parts; p += 4) s += part[p * N + col];
+    sums[q][c] = s;
+    __syncthreads();
+    if (q == 0 && col < N) db[col] = (T)(alpha * (sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]));
+}
+
+// ---- launches --------------------------------------------------------------------------------
+template <typename T, int BI, int BJ, int WI, int WJ>
+int launch_gemm(int role, bool vec, const GemmArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)(a.ti * a.tj * a.splits)), block(64 * WI * WJ);
+#define PSFM_LAUNCH(PT, QT, FULL)                                            \
+    (vec ? (void)(k_gemm<T, BI, BJ, WI, WJ, PT, QT, true, FULL><<<grid, block, 0, s>>>(a)) \
+         : (void)(k_gemm<T, BI, BJ, WI, WJ, PT, QT, false, FULL><<<grid, block, 0, s>>>(a)))
+    if (role == GEMM_FWD)
+        PSFM_LAUNCH(false, false, true);
+    else if (role == GEMM_DX)
+        PSFM_LAUNCH(false, true, false);
+    else
+        PSFM_LAUNCH(true, true, false);
+#undef PSFM_LAUNCH
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int gemm_of(int role, int variant, bool vec, const GemmArgs& a, hipStream_t s) {
+    return variant == 0 ? launch_gemm<T, 64, 64, 2, 2>(role, vec, a, s) : launch_gemm<T, 128, 128, 2, 2>(role, vec, a, s);
+}
+
+template <typename T>
+int join_of(const GemmArgs& a, bool full, hipStream_t s) {
+    const dim3 grid((unsigned)((a.I * ((a.J + 3) >> 2) + 255) / 256));
+    if (full)
+        k_join<T, true><<<grid, 256, 0, s>>>(a);
+    else
+        k_join<T, false><<<grid, 256, 0, s>>>(a);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int dz_of(const DzArgs& a, int64_t gx, int64_t gy, bool, hipStream_t s) {
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    k_dz<T, 16><<<grid, DZ_THREADS, 0, s>>>(a);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int colsum_of(const float* part, int64_t parts, int64_t N, float alpha, void* db, hipStream_t s) {
+    k_colsum<T><<<dim3((unsigned)((N + 63) / 64)), 256, 0, s>>>(part, parts, N, alpha, (T*)db);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+}  // namespace psfm

@@ -1,0 +1,217 @@
+"""Dropout from a counter-based generator (include/psfm_dropout.h, csrc/psfm_dropout.hip).
+
+The reference's ResidualConv drops whole channels of its shortcut (nn.Dropout2d,
+packnet_sfm/networks/layers/packnet/layers01.py:40-61).  Here a mask is a function of (seed, offset, position)
+(Philox4x32-10; the header says which word is whose), so the forward and the backward pass each make it
+again and neither stores it, and a run can be repeated from its seed whatever else drew random numbers:
+
+  dropout(x, drop, residual)     y = [residual +] x with dropped values 0 and kept ones times 1 / (1 - p),
+                                 columns along the last dimension
+  dropout2d(x, drop, residual)   the same on [B, C, H, W] images, columns along C
+  Drop(p, rng, channels)         one mask: probability, int64 pair (seed, offset) on x's device, and whether all
+                                 positions of a sample (the first dimension) share one row of it
+  CounterDropout(p, seed)        the module: draws a new offset on the device at every training forward
+
+linear.linear_act takes the same Drop into its epilogue: the mask is the one that `dropout` would
+give its output.  fp32, fp16 and bf16 tensors on a ROCm device run the HIP kernel; anything else
+(CPU tensors, fp64) runs the same arithmetic as plain torch ops.
+"""
+from contextlib import nullcontext
+from typing import NamedTuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ... import _hip
+
+
+class Drop(NamedTuple):
+    p: float
+    rng: torch.Tensor
+    channels: bool = False
+
+
+def check_drop(drop, device):
+    """Drop's arguments; returns it, or None where it drops nothing."""
+    p, rng, _ = drop
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability {p} is not in 0 .. 1")
+    if p == 0.0:
+        return None
+    if rng.dtype != torch.int64 or rng.numel() != 2 or rng.device != device or not rng.is_contiguous():
+        raise RuntimeError(f"rng must be a contiguous int64 pair (seed, offset) on {device}; got {rng.dtype} "
+                           f"{tuple(rng.shape)} on {rng.device}")
+    return drop
+
+
+def mask_rows(shape, channels):
+    """How many consecutive rows of a [..., columns] tensor share a row of the mask."""
+    if not channels:
+        return 1
+    n = 1
+    for s in shape[1:-1]:
+        n *= s
+    return max(n, 1)
+
+
+def row_stride(t):
+    """The stride between consecutive rows of t as a [rows, last dimension] matrix, or None where it has no
+    such form (columns apart, rows at uneven distances)."""
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return cols
+    if t.stride(-1) != 1 and cols != 1:
+        return None
+    ld = None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if ld is None:
+            ld, reach = stride, stride * size
+        elif stride == reach:
+            reach = stride * size
+        else:
+            return None
+    if ld is None:
+        return cols
+    return ld if ld >= cols else None
+
+
+def as_rows(t):
+    """(t, its row stride), copied only where it has none."""
+    ld = row_stride(t)
+    if ld is None:
+        t = t.contiguous()
+        ld = t.shape[-1]
+    return t, ld
+
+
+def on_device(t):
+    """Launches go to the current device: make it t's."""
+    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def keep_mask(rows, cols, p, rng):
+    """The kept values of a [rows, cols] mask, in plain torch integer operations on rng's device."""
+    blocks, low = (cols + 3) // 4, 0xFFFFFFFF
+    at = torch.arange(rows * blocks, device=rng.device)
+    c0, c1 = at & low, at >> 32
+    c2, c3 = (rng[1] & low).expand_as(at), (rng[1] >> 32 & low).expand_as(at)
+    k0, k1 = rng[0] & low, rng[0] >> 32 & low
+    for _ in range(10):
+        # 32 x 32 bits: the product wraps into int64's sign and keeps its bits
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = (b >> 32 & low) ^ c1 ^ k0, b & low, (a >> 32 & low) ^ c3 ^ k1, a & low
+        k0, k1 = k0 + 0x9E3779B9 & low, k1 + 0xBB67AE85 & low
+    words = torch.stack((c0, c1, c2, c3), 1).view(rows, 4 * blocks)[:, :cols]
+    return words >= int(p * 2.0 ** 32 + 0.5)
+
+
+def plain_drop(t, drop):
+    """dropout of t in plain torch operations."""
+    shape = t.shape
+    if t.numel() == 0:
+        return t
+    share = mask_rows(shape, drop.channels)
+    keep = keep_mask(t.numel() // shape[-1] // share, shape[-1], drop.p, drop.rng)
+    scale = 1.0 / (1.0 - drop.p) if drop.p < 1.0 else 0.0
+    return torch.where(keep.unsqueeze(1), t.reshape(-1, share, shape[-1]) * scale, 0.0).view(shape)
+
+
+def _launch(x, residual, p, rng, share):
+    x, ldx = as_rows(x)
+    res, ldr = (None, 0) if residual is None else as_rows(residual)
+    cols = x.shape[-1]
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if y.numel():
+        with on_device(x):
+            _hip.check(_hip.lib().psfm_dropout(_hip.ptr(x), ldx, _hip.ptr(res), ldr, _hip.DTYPES[x.dtype],
+                                               x.numel() // cols, cols, share, p, _hip.ptr(rng), _hip.ptr(y),
+                                               _hip.stream(x.device)), "psfm_dropout")
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, rng, share):
+        _hip.note_forward(ctx)
+        ctx.save_for_backward(rng)
+        ctx.p, ctx.share = p, share
+        return _launch(x, residual, p, rng, share)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _hip.capture_guard(ctx, leaves=True)
+        (rng,) = ctx.saved_tensors
+        dx = _launch(dy, None, ctx.p, rng, ctx.share) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def check_like(t, name, shape, x):
+    if t.shape != shape or t.dtype != x.dtype or t.device != x.device:
+        raise RuntimeError(f"{name} must be {tuple(shape)} {x.dtype} on {x.device}; got {tuple(t.shape)} {t.dtype} on "
+                           f"{t.device}")
+
+
+def dropout(x, drop, residual=None):
+    """[residual +] drop(x) over the last dimension's columns; drop None: nothing is dropped.  A dropped value is
+    0 whatever it was, infinities and NaN included.  The sum is taken in fp32 and rounded once."""
+    if x.dim() == 0:
+        raise RuntimeError("dropout needs at least one dimension")
+    if residual is not None:
+        check_like(residual, "residual", x.shape, x)
+    if drop is not None:
+        drop = check_drop(drop, x.device)
+    if drop is None:
+        return x if residual is None else x + residual
+    if not x.is_cuda or x.dtype not in _hip.DTYPES:
+        wide = torch.promote_types(x.dtype, torch.float32)
+        y = plain_drop(x.to(wide), drop)
+        return (y if residual is None else y + residual.to(wide)).to(x.dtype)
+    share = mask_rows(x.shape, drop.channels)
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
+        return _Dropout.apply(x, residual, drop.p, drop.rng, share)
+    return _launch(x, residual, drop.p, drop.rng, share)
+
+
+def dropout2d(x, drop, residual=None):
+    """dropout of [B, C, H, W] images with C as the mask's columns (channels_last storage is taken as it is); with
+    drop.channels whole channels of a sample are dropped, as nn.Dropout2d does."""
+    if x.dim() != 4:
+        raise RuntimeError(f"dropout2d takes [B, C, H, W] images, got {tuple(x.shape)}")
+    res = None if residual is None else residual.permute(0, 2, 3, 1)
+    return dropout(x.permute(0, 2, 3, 1), drop, res).permute(0, 3, 1, 2)
+
+
+class CounterDropout(nn.Module):
+    """Dropout whose masks are (seed, offset), the offset counted on the device: in training every forward draws
+    the next one, also in a captured graph's replays.  Data-parallel ranks and the layers of one network take
+    different seeds or first offsets.  The state is no part of the state_dict: checkpoints of networks with
+    nn.Dropout load as they are."""
+
+    def __init__(self, p, seed, offset=0, channels=False):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability {p} is not in 0 .. 1")
+        self.p, self.channels = float(p), channels
+        wrap = [(int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63 for v in (seed, offset)]
+        self.register_buffer("state", torch.tensor(wrap, dtype=torch.int64), persistent=False)
+
+    def draw(self):
+        """The Drop of this forward (None where nothing is dropped)."""
+        if not self.training or self.p == 0.0:
+            return None
+        if not self.state.is_cuda:
+            used = self.state.clone()
+            self.state[1] += 1
+            return Drop(self.p, used, self.channels)
+        used = torch.empty_like(self.state)
+        with on_device(self.state):
+            _hip.check(_hip.lib().psfm_rng_next(_hip.ptr(self.state), _hip.ptr(used), _hip.stream(self.state.device)),
+                       "psfm_rng_next")
+        return Drop(self.p, used, self.channels)
+
+    def forward(self, x, residual=None):
+        return (dropout2d if x.dim() == 4 else dropout)(x, self.draw(), residual)
