@@ -45,8 +45,9 @@ typedef struct psfm_linear {
 
 /* Workspace of the forward pass in bytes (0: none needed), or -1 (bad descriptor). */
 int64_t psfm_linear_fwd_ws_bytes(const psfm_linear* d);
-/* bias, res and z may be NULL.  z [M, N], in x's type, receives the values before the activation that the
- * backward pass differentiates at. */
+/* bias, res and z may be NULL.  z [M, N] receives the values before the activation, which the backward pass
+ * differentiates at: in x's type for PSFM_ACT_RELU, else in fp16 (clamped to its range) for bf16 and in fp32
+ * for fp16 and fp32 tensors. */
 int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const void* bias, const void* res, void* y,
                     void* z, void* ws, void* stream);
 

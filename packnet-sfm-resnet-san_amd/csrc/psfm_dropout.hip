@@ -2,10 +2,11 @@
 //
 //   y[r, c] = [res[r, c] +] (word(mask row, c) < p 2^32 ? 0 : x[r, c] / (1 - p))
 //
-// One thread takes four columns of a row, one Philox block.
+// One read of x and res, one write of y.  A thread takes chunks of 16 bytes (8 values of 16 bits: two Philox blocks),
+// UNROLL of them with their loads first; a workgroup's chunks are consecutive, so that one 64-bit division a
+// workgroup finds its first row and the threads go on in 32 bits.
 #include "../../include/psfm_dropout.h"
 
-#include <algorithm>
 #include <string>
 
 #include "psfm_philox.h"
@@ -35,26 +36,74 @@ struct Args {
     DropArgs drop;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_dropout(const Args A) {
-    const int64_t cb = (A.cols + 3) >> 2, total = A.rows * cb;
+constexpr int UNROLL = 4, THREADS = 256;
+
+template <typename T, bool RES>
+__global__ __launch_bounds__(THREADS) void k_dropout(const Args A) {
+    constexpr int V = 16 / (int)sizeof(T);
+    typedef T TV __attribute__((ext_vector_type(V)));
+    const int64_t cpr = (A.cols + V - 1) / V, first = (int64_t)blockIdx.x * THREADS * UNROLL, row0 = first / cpr;
+    const int64_t in0 = first - row0 * cpr;
     PhiloxKey key{};
     if (A.drop.rng) key = philox_key(A.drop.rng);
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < total; id += (int64_t)gridDim.x * 256) {
-        const int64_t r = id / cb, c = (id - r * cb) * 4;
-        const T* x = (const T*)A.x + r * A.ldx + c;
-        const T* res = A.res ? (const T*)A.res + r * A.ldr + c : nullptr;
-        T* y = (T*)A.y + r * A.cols + c;
-        uint32_t w[4];
-        if (A.drop.rng) philox4(key, mask_block(mask_row(A.drop, r), A.cols, c), w);
+    int64_t row[UNROLL], col[UNROLL];
+    TV x[UNROLL], res[UNROLL];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (c + k >= A.cols) continue;
-            float v = (float)x[k];
-            if (A.drop.rng) v = w[k] <= A.drop.last ? 0.0f : v * A.drop.scale;
-            y[k] = (T)(res ? v + (float)res[k] : v);
+    for (int u = 0; u < UNROLL; ++u) {
+        const int64_t at = in0 + u * THREADS + threadIdx.x;
+        const int64_t down = (cpr >> 31) == 0 ? (uint32_t)at / (uint32_t)cpr : at / cpr;
+        row[u] = row0 + down;
+        col[u] = (at - down * cpr) * V;
+        const bool whole = row[u] < A.rows && col[u] + V <= A.cols;
+        if (whole) {
+            __builtin_memcpy(&x[u], (const T*)A.x + row[u] * A.ldx + col[u], 16);
+            if (RES) __builtin_memcpy(&res[u], (const T*)A.res + row[u] * A.ldr + col[u], 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const bool in = row[u] < A.rows && col[u] + k < A.cols;
+                x[u][k] = in ? ((const T*)A.x)[row[u] * A.ldx + col[u] + k] : (T)0.0f;
+                if (RES) res[u][k] = in ? ((const T*)A.res)[row[u] * A.ldr + col[u] + k] : (T)0.0f;
+            }
         }
     }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        if (row[u] >= A.rows) return;
+        TV y;
+        const uint64_t block = A.drop.rng ? mask_block(mask_row(A.drop, row[u]), A.cols, col[u]) : 0;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            uint32_t w[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (A.drop.rng) philox4(key, block + q, w);
+#pragma unroll
+            for (int k = 4 * q; k < 4 * q + 4; ++k) {
+                float v = (float)x[u][k];
+                if (A.drop.rng) v = w[k & 3] <= A.drop.last ? 0.0f : v * A.drop.scale;
+                y[k] = (T)(RES ? v + (float)res[u][k] : v);
+            }
+        }
+        T* p = (T*)A.y + row[u] * A.cols + col[u];
+        if (col[u] + V <= A.cols) {
+            __builtin_memcpy(p, &y, 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (col[u] + k < A.cols) p[k] = y[k];
+        }
+    }
+}
+
+template <typename T>
+int run(const Args& a, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T), PER = THREADS * UNROLL;
+    const int64_t blocks = (a.rows * ((a.cols + V - 1) / V) + PER - 1) / PER;
+    if (blocks > 0x7fffffff) return fail(-1, "psfm_dropout: more values than a launch holds");
+    if (a.res)
+        k_dropout<T, true><<<dim3((unsigned)blocks), THREADS, 0, s>>>(a);
+    else
+        k_dropout<T, false><<<dim3((unsigned)blocks), THREADS, 0, s>>>(a);
+    return status("psfm_dropout: launch");
 }
 
 __global__ void k_rng_next(int64_t* state, int64_t* used) {
@@ -82,16 +131,8 @@ int psfm_dropout(const void* x, int64_t ldx, const void* res, int64_t ldr, int d
     if (ldx < cols || (res && ldr < cols)) return fail(-6, "psfm_dropout: a row stride below the row's length");
     Args a{x, res, y, ldx, ldr, rows, cols, DropArgs{nullptr, 0, 1.0f, 1}};
     if (p > 0.0 && drop_threshold(p, &a.drop.last, &a.drop.scale)) a.drop.rng = rng, a.drop.mask_rows = mask_rows;
-    const int64_t groups = rows * ((cols + 3) / 4);
-    const dim3 grid((unsigned)std::min<int64_t>((groups + 255) / 256, 16384));
     const hipStream_t s = (hipStream_t)stream;
-    if (dtype == PSFM_DTYPE_F32)
-        k_dropout<float><<<grid, 256, 0, s>>>(a);
-    else if (dtype == PSFM_DTYPE_F16)
-        k_dropout<_Float16><<<grid, 256, 0, s>>>(a);
-    else
-        k_dropout<__bf16><<<grid, 256, 0, s>>>(a);
-    return status("psfm_dropout: launch");
+    return dtype == PSFM_DTYPE_F32 ? run<float>(a, s) : dtype == PSFM_DTYPE_F16 ? run<_Float16>(a, s) : run<__bf16>(a, s);
 }
 
 int psfm_rng_next(int64_t* state, int64_t* used, void* stream) {

@@ -19,7 +19,6 @@ struct LinearEpi {
     int act;
     float alpha;
     DropArgs drop;
-    bool whole, whole_res; // four columns of out, z and bias (of res) from a multiple of four are one aligned access
 };
 
 // out[i, j] = sum over r of P[i, r] Q[j, r].  A "turned" operand is stored with r as its row.
@@ -45,15 +44,14 @@ struct DzArgs {
     int64_t M, N, rows;    // rows of one workgroup
     int act;
     DropArgs drop;
-    bool whole;            // as LinearEpi's, of dy, z and dz
 };
 
 // One set per type (psfm_linear_<type>.hip).  Each returns a hipError_t.
 struct LinearOps {
-    // tile edges of (role, variant); variant 0 is the smallest
+    // variant: an index into LINEAR_TILES
     int (*gemm)(int role, int variant, bool vec, const GemmArgs& a, hipStream_t s);
     int (*join)(const GemmArgs& a, bool full, hipStream_t s);
-    int (*dz)(const DzArgs& a, int64_t gx, int64_t gy, bool vec, hipStream_t s);
+    int (*dz)(const DzArgs& a, int64_t gx, int64_t gy, hipStream_t s);
     int (*colsum)(const float* part, int64_t parts, int64_t N, float alpha, void* db, hipStream_t s);
 };
 
@@ -68,5 +66,7 @@ struct Tile {
 constexpr Tile LINEAR_TILES[] = {{64, 64}, {128, 128}};
 constexpr int LINEAR_NTILES = 2;
 constexpr int DZ_THREADS = 256;
+// chunks of columns in a k_dz workgroup: all of a narrow layer's, 32 of a wide one's
+constexpr int DZ_NARROW = 8, DZ_WIDE = 32;
 
 }  // namespace psfm

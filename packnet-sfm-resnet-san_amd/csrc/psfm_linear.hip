@@ -81,10 +81,12 @@ int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 struct DzPlan {
     int64_t gx, gy, rows;
 };
-DzPlan dz_plan(int64_t M, int64_t N) {
+// About four workgroups a CU, each with a few rows a thread at least.
+DzPlan dz_plan(int dtype, int64_t M, int64_t N) {
     DzPlan p;
-    p.gx = up(N, 64);
-    p.gy = std::max<int64_t>(1, std::min({up(2048, std::max<int64_t>(p.gx, 1)), up(M, 64), (int64_t)65535}));
+    const int64_t v = 16 / size_of(dtype), cb = N <= DZ_NARROW * v ? DZ_NARROW : DZ_WIDE, rp = DZ_THREADS / cb;
+    p.gx = up(N, cb * v);
+    p.gy = std::max<int64_t>(1, std::min(up(1024, std::max<int64_t>(p.gx, 1)), up(M, 2 * rp)));
     p.rows = up(std::max<int64_t>(M, 1), p.gy);
     p.gy = up(std::max<int64_t>(M, 1), p.rows);
     return p;
@@ -94,18 +96,11 @@ bool mult(const void* p, int64_t ld, int64_t edge, int64_t v) {
     return ((uintptr_t)p & 15) == 0 && ld % v == 0 && edge % v == 0;
 }
 
-// four values from every multiple of four of every row are one aligned access
-bool fours(const void* p, int64_t ld, int dtype) {
-    return ((uintptr_t)p & (4 * size_of(dtype) - 1)) == 0 && (ld & 3) == 0;
-}
-
 int run_gemm(int role, int dtype, GemmArgs& a, const Plan& p, void* ws, hipStream_t s) {
     const int64_t v = 16 / size_of(dtype);
     const bool pt = role == GEMM_DW, qt = role != GEMM_FWD;
     const bool vec = mult(a.P, a.ldp, pt ? a.I : a.R, v) && mult(a.Q, a.ldq, qt ? a.J : a.R, v);
     if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear: more tiles than a launch holds");
-    a.e.whole = fours(a.e.out, a.J, dtype) && fours(a.e.z, a.J, dtype) && fours(a.e.bias, a.J, dtype);
-    a.e.whole_res = (a.J & 3) == 0 && fours(a.e.res, a.e.ldr, dtype);
     a.ti = (uint32_t)p.ti, a.tj = (uint32_t)p.tj, a.splits = p.splits, a.rsplit = p.rsplit, a.part = (float*)ws;
     const LinearOps& o = ops_of(dtype);
     int e = o.gemm(role, p.variant, vec, a, s);
@@ -122,7 +117,7 @@ struct BwdPlan {
 BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db) {
     BwdPlan b{};
     b.dz = (want_dx || want_dw) && (d->act != PSFM_ACT_NONE || drop_of(d).rng);
-    b.cols = dz_plan(d->M, d->N);
+    b.cols = dz_plan(d->dtype, d->M, d->N);
     b.dz_at = 0;
     b.cols_at = b.dz ? aligned(d->M * d->N * size_of(d->dtype)) : 0;
     b.parts_at = b.cols_at + (want_db ? aligned(b.cols.gy * d->N * 4) : 0);
@@ -152,7 +147,7 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
     if (part_bytes(p, d->M, d->N) > 0 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
     GemmArgs a{};
     a.P = x, a.Q = w, a.ldp = d->ldx, a.ldq = d->K, a.I = d->M, a.J = d->N, a.R = d->K;
-    a.e = LinearEpi{y, bias, res, d->ldr, z, d->act, 1.0f, drop_of(d), false, false};
+    a.e = LinearEpi{y, bias, res, d->ldr, z, d->act, 1.0f, drop_of(d)};
     return run_gemm(GEMM_FWD, d->dtype, a, p, ws, (hipStream_t)stream);
 }
 
@@ -177,9 +172,8 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
     const void* dz = b.dz ? ws : dy;
     if (any && (b.dz || db)) {
         const DzArgs a{dy, d->act != PSFM_ACT_NONE ? z : nullptr, b.dz ? ws : nullptr, db ? cols : nullptr,
-                       d->M, d->N, b.cols.rows, d->act, drop,
-                       fours(dy, d->N, d->dtype) && (d->act == PSFM_ACT_NONE || fours(z, d->N, d->dtype))};
-        if (const int rc = status(o.dz(a, b.cols.gx, b.cols.gy, false, s), "psfm_linear_bwd: dz launch")) return rc;
+                       d->M, d->N, b.cols.rows, d->act, drop};
+        if (const int rc = status(o.dz(a, b.cols.gx, b.cols.gy, s), "psfm_linear_bwd: dz launch")) return rc;
     }
     if (db && d->N > 0) {
         const int e = o.colsum(cols, any ? b.cols.gy : 0, d->N, drop.scale, db, s);

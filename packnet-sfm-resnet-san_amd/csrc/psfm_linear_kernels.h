@@ -23,36 +23,67 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 template <typename T>
 constexpr int CHUNK = 16 / (int)sizeof(T);   // values of one 16-byte chunk
 
-// ---- activations, in fp32 ---------------------------------------------------------------------
+// ---- activations, in fp32, of N values under one (uniform) choice ------------------------------
 __device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + __expf(-z)); }
 
-__device__ __forceinline__ float act_of(int act, float z) {
+template <int N>
+__device__ __forceinline__ void act_of(int act, float (&z)[N]) {
+#define PSFM_EACH(F)                         \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) { \
+        const float v = z[k];                \
+        z[k] = F;                            \
+    }                                        \
+    break;
     switch (act) {
-        case PSFM_ACT_RELU: return z < 0.0f ? 0.0f : z;     // NaN stays
-        case PSFM_ACT_SIGMOID: return sigmoidf(z);
-        case PSFM_ACT_ELU: return z > 0.0f ? z : expm1f(z);
-        case PSFM_ACT_SILU: return z / (1.0f + __expf(-z));
-        case PSFM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        default: return z;
+        case PSFM_ACT_RELU: PSFM_EACH(v < 0.0f ? 0.0f : v)     // NaN stays
+        case PSFM_ACT_SIGMOID: PSFM_EACH(sigmoidf(v))
+        case PSFM_ACT_ELU: PSFM_EACH(v > 0.0f ? v : expm1f(v))
+        case PSFM_ACT_SILU: PSFM_EACH(v / (1.0f + __expf(-v)))
+        case PSFM_ACT_GELU: PSFM_EACH(0.5f * v * (1.0f + erff(v * 0.70710678118654752f)))
+        default: break;
     }
+#undef PSFM_EACH
 }
-__device__ __forceinline__ float slope_of(int act, float z) {
+
+__device__ __forceinline__ float slope_silu(float z) {
+    const float s = sigmoidf(z);
+    return s * (1.0f + z * (1.0f - s));
+}
+__device__ __forceinline__ float slope_sigmoid(float z) {
+    const float s = sigmoidf(z);
+    return s * (1.0f - s);
+}
+__device__ __forceinline__ float slope_gelu(float z) {
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+}
+template <int N>
+__device__ __forceinline__ void times_slope(int act, const float (&z)[N], float (&d)[N]) {
+#define PSFM_EACH(F) \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) d[k] *= F; \
+    break;
     switch (act) {
-        case PSFM_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case PSFM_ACT_SIGMOID: {
-            const float s = sigmoidf(z);
-            return s * (1.0f - s);
-        }
-        case PSFM_ACT_ELU: return z > 0.0f ? 1.0f : __expf(z);
-        case PSFM_ACT_SILU: {
-            const float s = sigmoidf(z);
-            return s * (1.0f + z * (1.0f - s));
-        }
-        case PSFM_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
-        default: return 1.0f;
+        case PSFM_ACT_RELU: PSFM_EACH((z[k] > 0.0f ? 1.0f : 0.0f))
+        case PSFM_ACT_SIGMOID: PSFM_EACH(slope_sigmoid(z[k]))
+        case PSFM_ACT_ELU: PSFM_EACH((z[k] > 0.0f ? 1.0f : __expf(z[k])))
+        case PSFM_ACT_SILU: PSFM_EACH(slope_silu(z[k]))
+        case PSFM_ACT_GELU: PSFM_EACH(slope_gelu(z[k]))
+        default: break;
     }
+#undef PSFM_EACH
 }
+
+// What z is kept in for the backward pass.  The slope is taken at it, so its rounding adds to dz's own: in bf16 that
+// made the gradients of sigmoid 1.7 times as far from 64 bits as one rounding.  fp16 has 8 times
+// bf16's steps in the same bytes; beyond its range (+-65504) every slope has reached its limit.  fp16
+// products keep z in fp32.  ReLU needs the sign alone, in the type itself.
+template <typename T>
+struct KeptZ {
+    using type = float;
+};
+template <>
+struct KeptZ<__bf16> {
+    using type = _Float16;
+};
 
 // ---- chunks of up to 16 bytes at any alignment that the type has -------------------------------
 template <typename T>
@@ -83,66 +114,89 @@ __device__ __forceinline__ u4v load_n(const T* p, int n) {
     return VEC ? u4v{0, 0, 0, 0} : load_part(p, n);
 }
 
-// ---- the epilogue of four consecutive columns j .. j + 3 (n of them exist) of row i ------------
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float v[4], int n, bool whole) {
-    if (whole) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<T4*>(p) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+// ---- runs of N consecutive values, the first n of them there, at any alignment that the type has ---
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T* p, const float (&v)[N], int n) {
+    typedef T TN __attribute__((ext_vector_type(N)));
+    if (n >= N) {
+        TN t;
+#pragma unroll
+        for (int k = 0; k < N; ++k) t[k] = (T)v[k];
+        __builtin_memcpy(p, &t, sizeof(T) * N);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < N; ++k)
             if (k < n) p[k] = (T)v[k];
     }
 }
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float v[4], int n, bool whole) {
-    if (whole) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const T4 t = *reinterpret_cast<const T4*>(p);
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, float (&v)[N], int n) {
+    typedef T TN __attribute__((ext_vector_type(N)));
+    if (n >= N) {
+        TN t;
+        __builtin_memcpy(&t, p, sizeof(T) * N);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = (float)t[k];
+        for (int k = 0; k < N; ++k) v[k] = (float)t[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = k < n ? (float)p[k] : 0.0f;
+        for (int k = 0; k < N; ++k) v[k] = k < n ? (float)p[k] : 0.0f;
     }
 }
 
-// mrow: row i's mask row
-template <typename T, bool FULL>
-__device__ __forceinline__ void epilogue4(const LinearEpi& e, const PhiloxKey& key, int64_t J, int64_t i, int64_t mrow,
-                                          int64_t j, float v[4]) {
-    const int n = J - j < 4 ? (int)(J - j) : 4;
-    const bool whole = e.whole;
+// v[k] = kept ? v[k] * scale : 0 for the columns j .. j + N - 1 (j % 4 = 0) of mask row mrow
+template <int N>
+__device__ __forceinline__ void drop_run(const DropArgs& d, const PhiloxKey& key, int64_t cols, int64_t mrow, int64_t j,
+                                         float scale, float (&v)[N]) {
+    const uint64_t block = mask_block(mrow, cols, j);
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        uint32_t w[4];
+        philox4(key, block + q, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * q + k] = w[k] <= d.last ? 0.0f : v[4 * q + k] * scale;
+    }
+}
+
+// ---- the epilogue of columns j .. j + N - 1 (j % 4 = 0; those below J exist) of row i -----------------
+template <typename T, bool FULL, int N>
+__device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& key, int64_t J, int64_t i, int64_t j,
+                                         float (&v)[N]) {
+    const int n = J - j < N ? (int)(J - j) : N;
     const int64_t at = i * J + j;
     if (!FULL) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] *= e.alpha;
-        store4((T*)e.out + at, v, n, whole);
+        for (int k = 0; k < N; ++k) v[k] *= e.alpha;
+        store_run((T*)e.out + at, v, n);
         return;
     }
     if (e.bias) {
-        float b[4];
-        load4((const T*)e.bias + j, b, n, whole);
+        float b[N];
+        load_run((const T*)e.bias + j, b, n);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += b[k];
+        for (int k = 0; k < N; ++k) v[k] += b[k];
     }
-    if (e.z) store4((T*)e.z + at, v, n, whole);
+    if (e.z) {
+        using Z = typename KeptZ<T>::type;
+        if (e.act == PSFM_ACT_RELU) {
+            store_run((T*)e.z + at, v, n);
+        } else if (sizeof(Z) == 2) {
+            float c[N];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = act_of(e.act, v[k]);
-    if (e.drop.rng) {
-        uint32_t w[4];
-        philox4(key, mask_block(mrow, J, j), w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = w[k] <= e.drop.last ? 0.0f : v[k] * e.drop.scale;
+            for (int k = 0; k < N; ++k) c[k] = v[k] != v[k] ? v[k] : fminf(fmaxf(v[k], -65504.0f), 65504.0f);
+            store_run((Z*)e.z + at, c, n);
+        } else {
+            store_run((Z*)e.z + at, v, n);
+        }
     }
+    act_of(e.act, v);
+    if (e.drop.rng) drop_run(e.drop, key, J, mask_row(e.drop, i), j, e.drop.scale, v);
     if (e.res) {
-        float r[4];
-        load4((const T*)e.res + i * e.ldr + j, r, n, e.whole_res);
+        float r[N];
+        load_run((const T*)e.res + i * e.ldr + j, r, n);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += r[k];
+        for (int k = 0; k < N; ++k) v[k] += r[k];
     }
-    store4((T*)e.out + at, v, n, whole);
+    store_run((T*)e.out + at, v, n);
 }
 
 // ---- LDS images ----------------------------------------------------------------------------
@@ -293,103 +347,156 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm(const GemmArgs A) {
     }
 
     const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
-    PhiloxKey key{};
-    if (FULL && A.e.drop.rng && A.splits == 1) key = philox_key(A.e.drop.rng);
+    if (A.splits > 1) {
+#pragma unroll
+        for (int a = 0; a < SI; ++a) {
+            const int64_t i = i0 + wi * (BI / WI) + a * 16 + n;
+#pragma unroll
+            for (int b = 0; b < SJ; ++b) {
+                const int64_t j = j0 + wj * (BJ / WJ) + b * 16 + 4 * g;
+                if (i >= A.I || j >= A.J) continue;
+                const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+                store_run(A.part + (split * A.I + i) * A.J + j, v, A.J - j < 4 ? (int)(A.J - j) : 4);
+            }
+        }
+        return;
+    }
+    // The epilogue reads the tile back from LDS, 16 bytes of output a thread and whole row segments a wave, in a
+    // short loop: unrolled over the accumulators it was 64 copies of the activations and generators, and the
+    // instruction fetch took four times the product (silu at 4096 x 8192 x 2048: 884 us, 185 without it).
+    // 16-byte chunks are XORed by the row: the 16 rows of a store hit 16 bank quads.
+    constexpr int V = CHUNK<T>, CPR = BJ / V, RPP = NTH / CPR;
+    static_assert(BI * BJ * 4 <= (int)sizeof(smem) && NTH % CPR == 0 && BI % RPP == 0, "epilogue tile");
+    float* tile = reinterpret_cast<float*>(&smem[0][0]);
 #pragma unroll
     for (int a = 0; a < SI; ++a) {
-        const int64_t i = i0 + wi * (BI / WI) + a * 16 + n;
-        if (i >= A.I) continue;
-        const int64_t mrow = FULL ? mask_row(A.e.drop, i) : 0;
+        const int i = wi * (BI / WI) + a * 16 + n;
 #pragma unroll
         for (int b = 0; b < SJ; ++b) {
-            const int64_t j = j0 + wj * (BJ / WJ) + b * 16 + 4 * g;
-            if (j >= A.J) continue;
-            float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-            if (A.splits > 1)
-                store4(A.part + (split * A.I + i) * A.J + j, v, A.J - j < 4 ? (int)(A.J - j) : 4, (A.J & 3) == 0);
-            else
-                epilogue4<T, FULL>(A.e, key, A.J, i, mrow, j, v);
+            const int c = (wj * (BJ / WJ) + b * 16) / 4 + g;
+            *reinterpret_cast<f4*>(tile + i * BJ + ((c ^ (i & 15)) << 2)) = acc[a][b];
         }
     }
-}
-
-// One thread: four columns of one row, summed over the splits in order.
-template <typename T, bool FULL>
-__global__ __launch_bounds__(256) void k_join(const GemmArgs A) {
-    // a split product is small: its 4-column groups are counted in 32 bits
-    const uint32_t cb = (uint32_t)((A.J + 3) >> 2), id = blockIdx.x * 256 + threadIdx.x, row = id / cb;
-    if (row >= A.I) return;
-    const int64_t i = row, j = (int64_t)(id - row * cb) * 4;
-    const int n = A.J - j < 4 ? (int)(A.J - j) : 4;
-    float v[4] = {0, 0, 0, 0};
-    for (int s = 0; s < A.splits; ++s) {
-        float p[4];
-        load4(A.part + (s * A.I + i) * A.J + j, p, n, (A.J & 3) == 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += p[k];
-    }
+    __syncthreads();
     PhiloxKey key{};
     if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
-    epilogue4<T, FULL>(A.e, key, A.J, i, FULL ? mask_row(A.e.drop, i) : 0, j, v);
+    const int col = threadIdx.x % CPR * V;
+    if (j0 + col >= A.J) return;
+#pragma unroll 1
+    for (int i = threadIdx.x / CPR; i < BI && i0 + i < A.I; i += RPP) {
+        float v[V];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const f4 t = *reinterpret_cast<const f4*>(tile + i * BJ + (((col / 4 + q) ^ (i & 15)) << 2));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[4 * q + k] = t[k];
+        }
+        epilogue<T, FULL>(A.e, key, A.J, i0 + i, j0 + col, v);
+    }
 }
 
-// Workgroup (x, y): 4-column groups x * CB .. of rows y * rows ..; 256 / CB rows at a time.
+// Split products: 256 / SL groups of four columns a workgroup, SL threads a group, each summing every SL-th split;
+// the SL sums are added in order, then the same epilogue.
+template <typename T, bool FULL, int SL>
+__global__ __launch_bounds__(256) void k_join(const GemmArgs A) {
+    constexpr int G = 256 / SL;
+    __shared__ f4 sums[SL][G];
+    // a split product is small: its groups are counted in 32 bits
+    const uint32_t cb = (uint32_t)((A.J + 3) >> 2), q = threadIdx.x % G, lane = threadIdx.x / G,
+                   id = blockIdx.x * G + q, row = id / cb;
+    const int64_t i = row, j = (int64_t)(id - row * cb) * 4;
+    const int n = A.J - j < 4 ? (int)(A.J - j) : 4;
+    const bool in = row < A.I;
+    float v[4] = {0, 0, 0, 0};
+    if (in) {
+        const float* p = A.part + i * A.J + j;
+#pragma unroll 4
+        for (int s = lane; s < A.splits; s += SL) {
+            float t[4];
+            load_run(p + (int64_t)s * A.I * A.J, t, n);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += t[k];
+        }
+    }
+    if (SL > 1) {
+        sums[lane][q] = f4{v[0], v[1], v[2], v[3]};
+        __syncthreads();
+        if (lane) return;
+        for (int s = 1; s < SL; ++s)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += sums[s][q][k];
+    }
+    if (!in) return;
+    PhiloxKey key{};
+    if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
+    epilogue<T, FULL>(A.e, key, A.J, i, j, v);
+}
+
+// Workgroup (x, y): CB chunks of columns from x * CB, rows y * rows ..; 256 / CB rows at a time.
 template <typename T, int CB>
 __global__ __launch_bounds__(DZ_THREADS) void k_dz(const DzArgs A) {
-    constexpr int RP = DZ_THREADS / CB;
-    __shared__ float sums[RP][CB * 4];
+    constexpr int RP = DZ_THREADS / CB, V = CHUNK<T>;
+    __shared__ float sums[RP][CB * V];
     const int cx = threadIdx.x % CB, ry = threadIdx.x / CB;
-    const int64_t j = ((int64_t)blockIdx.x * CB + cx) * 4;
-    const int n = A.N - j < 4 ? (int)(A.N - j) : 4;
-    const bool whole = A.whole;
+    const int64_t j = ((int64_t)blockIdx.x * CB + cx) * V;
+    const int n = A.N - j < V ? (int)(A.N - j) : V;
     const int64_t m0 = (int64_t)blockIdx.y * A.rows, m1 = m0 + A.rows < A.M ? m0 + A.rows : A.M;
     PhiloxKey key{};
     if (A.drop.rng) key = philox_key(A.drop.rng);
-    float sum[4] = {0, 0, 0, 0};
+    float sum[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] = 0;
     if (n > 0) {
         for (int64_t m = m0 + ry; m < m1; m += RP) {
-            float d[4], zv[4];
-            load4((const T*)A.dy + m * A.N + j, d, n, whole);
-            if (A.z) load4((const T*)A.z + m * A.N + j, zv, n, whole);
+            float d[V];
+            load_run((const T*)A.dy + m * A.N + j, d, n);
             if (A.z) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) d[k] *= slope_of(A.act, zv[k]);
+                float z[V];
+                if (A.act == PSFM_ACT_RELU)
+                    load_run((const T*)A.z + m * A.N + j, z, n);
+                else
+                    load_run((const typename KeptZ<T>::type*)A.z + m * A.N + j, z, n);
+                times_slope(A.act, z, d);
             }
-            if (A.drop.rng) {   // last: a dropped value is 0 whatever dy and z hold
-                uint32_t w[4];
-                philox4(key, mask_block(mask_row(A.drop, m), A.N, j), w);
+            // last: a dropped value is 0 whatever dy and z hold
+            if (A.drop.rng) drop_run(A.drop, key, A.N, mask_row(A.drop, m), j, 1.0f, d);
+            if (A.dz) store_run((T*)A.dz + m * A.N + j, d, n);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) d[k] = w[k] <= A.drop.last ? 0.0f : d[k];
-            }
-            if (A.dz) store4((T*)A.dz + m * A.N + j, d, n, whole);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) sum[k] += d[k];
+            for (int k = 0; k < V; ++k) sum[k] += d[k];
         }
     }
     if (!A.part) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sums[ry][cx * 4 + k] = sum[k];
+    for (int k = 0; k < V; ++k) sums[ry][cx * V + k] = sum[k];
     __syncthreads();
-    for (int c = threadIdx.x; c < CB * 4; c += DZ_THREADS) {
-        const int64_t col = (int64_t)blockIdx.x * CB * 4 + c;
+    for (int c = threadIdx.x; c < CB * V; c += DZ_THREADS) {
+        const int64_t col = (int64_t)blockIdx.x * CB * V + c;
         if (col >= A.N) continue;
         float s = 0;
+#pragma unroll
         for (int r = 0; r < RP; ++r) s += sums[r][c];
         A.part[blockIdx.y * A.N + col] = s;
     }
 }
 
+// 16 columns a workgroup, 64 threads a column, each summing every 64th part; the 64 sums are added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_colsum(const float* part, int64_t parts, int64_t N, float alpha, T* db) {
-    __shared__ float sums[4][64];
-    const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+__global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t parts, int64_t N, float alpha, T* db) {
+    __shared__ float sums[64][17];
+    const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c;
     float s = 0;
-    if (col < N)
-        for (int64_t p = q; p < parts; p += 4) s += part[p * N + col];
+    if (col < N) {
+#pragma unroll 4
+        for (int64_t p = q; p < parts; p += 64) s += part[p * N + col];
+    }
     sums[q][c] = s;
     __syncthreads();
-    if (q == 0 && col < N) db[col] = (T)(alpha * (sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]));
+    if (q || col >= N) return;
+    s = 0;
+#pragma unroll
+    for (int r = 0; r < 64; ++r) s += sums[r][c];
+    db[col] = (T)(alpha * s);
 }
 
 // ---- launches --------------------------------------------------------------------------------
@@ -414,26 +521,33 @@ int gemm_of(int role, int variant, bool vec, const GemmArgs& a, hipStream_t s) {
     return variant == 0 ? launch_gemm<T, 64, 64, 2, 2>(role, vec, a, s) : launch_gemm<T, 128, 128, 2, 2>(role, vec, a, s);
 }
 
+template <typename T, bool FULL>
+void launch_join(const GemmArgs& a, hipStream_t s) {
+    const int64_t groups = a.I * ((a.J + 3) >> 2);
+    if (a.splits <= 8)   // few enough for one thread a group
+        k_join<T, FULL, 1><<<dim3((unsigned)((groups + 255) / 256)), 256, 0, s>>>(a);
+    else
+        k_join<T, FULL, 16><<<dim3((unsigned)((groups + 15) / 16)), 256, 0, s>>>(a);
+}
 template <typename T>
 int join_of(const GemmArgs& a, bool full, hipStream_t s) {
-    const dim3 grid((unsigned)((a.I * ((a.J + 3) >> 2) + 255) / 256));
-    if (full)
-        k_join<T, true><<<grid, 256, 0, s>>>(a);
-    else
-        k_join<T, false><<<grid, 256, 0, s>>>(a);
+    full ? launch_join<T, true>(a, s) : launch_join<T, false>(a, s);
     return (int)hipGetLastError();
 }
 
 template <typename T>
-int dz_of(const DzArgs& a, int64_t gx, int64_t gy, bool, hipStream_t s) {
+int dz_of(const DzArgs& a, int64_t gx, int64_t gy, hipStream_t s) {
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    k_dz<T, 16><<<grid, DZ_THREADS, 0, s>>>(a);
+    if (a.N <= DZ_NARROW * CHUNK<T>)
+        k_dz<T, DZ_NARROW><<<grid, DZ_THREADS, 0, s>>>(a);
+    else
+        k_dz<T, DZ_WIDE><<<grid, DZ_THREADS, 0, s>>>(a);
     return (int)hipGetLastError();
 }
 
 template <typename T>
 int colsum_of(const float* part, int64_t parts, int64_t N, float alpha, void* db, hipStream_t s) {
-    k_colsum<T><<<dim3((unsigned)((N + 63) / 64)), 256, 0, s>>>(part, parts, N, alpha, (T*)db);
+    k_colsum<T><<<dim3((unsigned)((N + 15) / 16)), 1024, 0, s>>>(part, parts, N, alpha, (T*)db);
     return (int)hipGetLastError();
 }
 

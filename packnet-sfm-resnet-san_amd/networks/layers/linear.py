@@ -26,6 +26,10 @@ _PLAIN = {ACT_NONE: lambda z: z, ACT_RELU: torch.relu, ACT_SIGMOID: torch.sigmoi
           ACT_GELU: F.gelu}
 
 
+# what the values before the activation are kept in (psfm_linear_fwd's z; ReLU's: the tensors' own type)
+_Z = {torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
+
+
 def _desc(x, ldx, ldr, N, act, p, rng, share):
     K = x.shape[-1]
     M = x.numel() // K if K else x.shape[:-1].numel()
@@ -43,7 +47,7 @@ def _forward(x, weight, bias, residual, act, p, rng, share, want_z):
     d = _desc(x, ldx, ldr, N, act, p, rng, share)
     L = _hip.lib()
     y = torch.empty(shape, device=x.device, dtype=x.dtype)
-    z = torch.empty(shape, device=x.device, dtype=x.dtype) if want_z else None
+    z = torch.empty(shape, device=x.device, dtype=x.dtype if act == ACT_RELU else _Z[x.dtype]) if want_z else None
     n = L.psfm_linear_fwd_ws_bytes(ctypes.byref(d))
     if n < 0:
         _hip.check(-1, "psfm_linear_fwd_ws_bytes")
@@ -56,9 +60,8 @@ def _forward(x, weight, bias, residual, act, p, rng, share, want_z):
 
 
 class _LinearAct(torch.autograd.Function):
-    """Saves x, the weight and the values before the activation, rounded to x's type (a second rounding of the
-    slope's argument, half the memory of fp32).  ReLU's slope is the sign of its output where nothing
-    follows it."""
+    """Saves x, the weight and the values before the activation (_Z).  ReLU's slope is the sign of its output
+    where nothing follows it."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, p, rng, share):
