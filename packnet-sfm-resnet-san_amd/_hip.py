@@ -369,7 +369,7 @@ def note_forward(ctx):
     capture (with its stream) until its backward runs (capture_guard(ctx))."""
     if not torch.cuda.is_initialized() or torch.cuda.is_current_stream_capturing():
         return
-    ctx._psfm_stream = torch.cuda.current_stream().cuda_stream
+    ctx._psfm_stream = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     with _CAPTURE_LOCK:
         _EAGER_CTX.add(ctx)
 
@@ -436,7 +436,8 @@ def stream(device):
     (PyTorch-ROCm runs a node's backward on its forward's stream) — HIP would otherwise record
     nothing for it and segfault in capture_end."""
     capture_guard()
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index))
 
 
 def tiles_per_image(H, W):

@@ -21,6 +21,16 @@ struct LinearEpi {
     DropArgs drop;
 };
 
+// dz = drop(dy) act'(z), made where dy is staged (z null: act' = 1).  `cols` receives the sums over m of each split of the
+// weight gradient, [splits, N], or `db` them scaled where there is one split.
+struct DzArgs {
+    const void* z;
+    int act;
+    DropArgs drop;
+    float* cols;
+    void* db;
+};
+
 // out[i, j] = sum over r of P[i, r] Q[j, r].  A "turned" operand is stored with r as its row.
 struct GemmArgs {
     const void* P;
@@ -32,27 +42,51 @@ struct GemmArgs {
     int splits;
     float* part;           // [splits, I, J] where splits > 1
     LinearEpi e;
+    DzArgs dz;
+    uint32_t blocks() const { return ti * tj * (uint32_t)splits; }
 };
 
-enum GemmRole { GEMM_FWD = 0, GEMM_DX = 1, GEMM_DW = 2 };   // (P, Q): (x, W), (dz, W turned), (dz turned, x turned)
+// A few rows times W, no tiles: y of 16 columns a workgroup
+struct SkinnyArgs {
+    const void* x;
+    const void* w;
+    int64_t ldx, M, N, K;
+    LinearEpi e;
+};
 
-struct DzArgs {
+// Both gradients' products in one launch: workgroups 0 .. dx.blocks() - 1 make dx, the rest dw.
+struct PairArgs {
+    GemmArgs dx, dw;
+    uint32_t ndx, ndw;
+};
+
+// What follows them in one launch: the joins of split products, then the column sums' parts.
+struct FinishArgs {
+    GemmArgs dx, dw;
+    uint32_t ndx, ndw, ncol;
+    const float* cols;
+    int64_t parts, N;
+    float alpha;
+    void* db;
+};
+
+// dz as a pass of its own
+struct DzPassArgs {
     const void* dy;
-    const void* z;         // null: act' = 1
-    void* dz;              // null: column sums only
-    float* part;           // [gridDim.y, N] column sums, or null
+    void* out;             // null: column sums only
     int64_t M, N, rows;    // rows of one workgroup
-    int act;
-    DropArgs drop;
+    DzArgs dz;             // cols: [gridDim.y, N] or null
 };
 
-// One set per type (psfm_linear_<type>.hip).  Each returns a hipError_t.
+// One set per type (psfm_linear_<type>.hip).  Each launches and returns a hipError_t; `variant` is an index into
+// LINEAR_TILES, `vec`: rows and runs of whole aligned 16-byte chunks.
 struct LinearOps {
-    // variant: an index into LINEAR_TILES
-    int (*gemm)(int role, int variant, bool vec, const GemmArgs& a, hipStream_t s);
-    int (*join)(const GemmArgs& a, bool full, hipStream_t s);
-    int (*dz)(const DzArgs& a, int64_t gx, int64_t gy, hipStream_t s);
-    int (*colsum)(const float* part, int64_t parts, int64_t N, float alpha, void* db, hipStream_t s);
+    int (*forward)(int variant, bool vec, const GemmArgs& a, hipStream_t s);
+    int (*join)(const GemmArgs& a, hipStream_t s);          // of a split forward
+    int (*skinny)(bool vec, const SkinnyArgs& a, hipStream_t s);
+    int (*pair)(int variant, bool vec, bool dz, const PairArgs& a, hipStream_t s);
+    int (*finish)(FinishArgs& a, hipStream_t s);
+    int (*dz)(const DzPassArgs& a, int64_t gx, int64_t gy, hipStream_t s);
 };
 
 const LinearOps& linear_ops_f32();
@@ -62,11 +96,11 @@ const LinearOps& linear_ops_bf16();
 struct Tile {
     int bi, bj;
 };
-// the tiles that every type is built for
-constexpr Tile LINEAR_TILES[] = {{64, 64}, {128, 128}};
-constexpr int LINEAR_NTILES = 2;
+constexpr Tile LINEAR_TILES[] = {{64, 64}, {128, 128}, {256, 256}};
+constexpr int LINEAR_NTILES = 3;   // 32-bit types: the first two
 constexpr int DZ_THREADS = 256;
 // chunks of columns in a k_dz workgroup: all of a narrow layer's, 32 of a wide one's
 constexpr int DZ_NARROW = 8, DZ_WIDE = 32;
+constexpr int SKINNY_ROWS = 32;    // at most
 
 }  // namespace psfm

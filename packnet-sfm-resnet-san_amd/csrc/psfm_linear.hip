@@ -58,13 +58,13 @@ struct Plan {
     int64_t blocks() const { return ti * tj * splits; }
 };
 
-// Tiles: the large one once it fills the 256 CUs, else the small one.  The reduction is split while the tiles
-// alone leave CUs idle and a split keeps at least four LDS stages.
-Plan plan(int dtype, int64_t I, int64_t J, int64_t R) {
+// Tiles: the largest that still fills the 256 CUs, else the smallest.  The reduction is split while the tiles alone
+// leave CUs idle and a split keeps at least four LDS stages.
+Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int variant = -1) {
     Plan p{0, 0, 0, 0, 1};
-    for (int v = LINEAR_NTILES - 1; v >= 0; --v) {
+    for (int v = variant >= 0 ? variant : dtype == PSFM_DTYPE_F32 ? 1 : 2; v >= 0; --v) {
         p.variant = v, p.ti = up(I, LINEAR_TILES[v].bi), p.tj = up(J, LINEAR_TILES[v].bj);
-        if (p.ti * p.tj >= 256) break;
+        if (p.ti * p.tj >= 256 || v == variant) break;
     }
     const int64_t stage = 128 / size_of(dtype), stages = up(R, stage), tiles = p.ti * p.tj;
     int64_t splits = 1;
@@ -77,6 +77,11 @@ Plan plan(int dtype, int64_t I, int64_t J, int64_t R) {
 
 int64_t part_bytes(const Plan& p, int64_t I, int64_t J) { return p.splits > 1 ? p.splits * I * J * 4 : 0; }
 int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+bool mult(const void* p, int64_t ld, int64_t edge, int64_t v) {
+    return ((uintptr_t)p & 15) == 0 && ld % v == 0 && edge % v == 0;
+}
+
+bool skinny(const psfm_linear* d) { return d->M <= SKINNY_ROWS; }
 
 struct DzPlan {
     int64_t gx, gy, rows;
@@ -92,40 +97,45 @@ DzPlan dz_plan(int dtype, int64_t M, int64_t N) {
     return p;
 }
 
-bool mult(const void* p, int64_t ld, int64_t edge, int64_t v) {
-    return ((uintptr_t)p & 15) == 0 && ld % v == 0 && edge % v == 0;
-}
-
-int run_gemm(int role, int dtype, GemmArgs& a, const Plan& p, void* ws, hipStream_t s) {
-    const int64_t v = 16 / size_of(dtype);
-    const bool pt = role == GEMM_DW, qt = role != GEMM_FWD;
-    const bool vec = mult(a.P, a.ldp, pt ? a.I : a.R, v) && mult(a.Q, a.ldq, qt ? a.J : a.R, v);
-    if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear: more tiles than a launch holds");
-    a.ti = (uint32_t)p.ti, a.tj = (uint32_t)p.tj, a.splits = p.splits, a.rsplit = p.rsplit, a.part = (float*)ws;
-    const LinearOps& o = ops_of(dtype);
-    int e = o.gemm(role, p.variant, vec, a, s);
-    if (e == 0 && p.splits > 1) e = o.join(a, role == GEMM_FWD, s);
-    return status(e, "psfm_linear: launch");
-}
-
 struct BwdPlan {
-    bool dz;          // dz has to be made (an activation or a mask); else it is dy
-    int64_t dz_at, cols_at, parts_at, bytes;
-    Plan dx, dw;
+    bool dx, dw;       // products to take (a wanted gradient of no values is none)
+    bool stage;        // the products make dz from dy as they stage it
+    bool pass;         // dz, or the column sums alone, as a pass of its own
+    bool dz;           // ... which writes dz
+    int64_t parts;     // of the column sums (0: the product writes db itself)
+    int64_t cols_at, dxp_at, dwp_at, bytes;
+    Plan pdx, pdw;
     DzPlan cols;
 };
+
+// The products share a launch where they share a tile.  They make dz themselves where that repeats little: every tile
+// column of either makes it once, and a pass of its own costs a launch and dz's way to memory and back.
 BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db) {
     BwdPlan b{};
-    b.dz = (want_dx || want_dw) && (d->act != PSFM_ACT_NONE || drop_of(d).rng);
+    const bool any = d->M > 0 && d->N > 0, make = d->act != PSFM_ACT_NONE || drop_of(d).rng;
+    b.dx = want_dx && d->M > 0 && d->K > 0;
+    b.dw = want_dw && d->N > 0 && d->K > 0;
+    if (b.dx) b.pdx = plan(d->dtype, d->M, d->K, d->N);
+    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M);
+    // at the largest tile the instances that make dz are not built: their columns are many
+    const int64_t columns = (b.dx ? b.pdx.tj : 0) + (b.dw ? b.pdw.tj : 0);
+    const bool large = (b.dx && b.pdx.variant > 1) || (b.dw && b.pdw.variant > 1);
+    const bool cheap = columns <= 4 || (double)columns * (double)d->M * (double)d->N < 8e6;
+    b.stage = any && (b.dx || b.dw) && !large && cheap && (make || (want_db && b.dw));
+    b.pass = any && !b.stage && ((make && (b.dx || b.dw)) || want_db);
+    if (b.stage && want_db && !b.dw) b.pass = true;      // the column sums alone
+    b.dz = b.pass && !b.stage && make && (b.dx || b.dw);
     b.cols = dz_plan(d->dtype, d->M, d->N);
-    b.dz_at = 0;
+    b.parts = !want_db || !any ? 0 : b.pass ? b.cols.gy : b.pdw.splits > 1 ? b.pdw.splits : 0;
     b.cols_at = b.dz ? aligned(d->M * d->N * size_of(d->dtype)) : 0;
-    b.parts_at = b.cols_at + (want_db ? aligned(b.cols.gy * d->N * 4) : 0);
-    int64_t parts = 0;
-    if (want_dx) b.dx = plan(d->dtype, d->M, d->K, d->N), parts = std::max(parts, part_bytes(b.dx, d->M, d->K));
-    if (want_dw) b.dw = plan(d->dtype, d->N, d->K, d->M), parts = std::max(parts, part_bytes(b.dw, d->N, d->K));
-    b.bytes = b.parts_at + parts;
+    b.dxp_at = b.cols_at + aligned(b.parts * d->N * 4);
+    b.dwp_at = b.dxp_at + (b.dx ? aligned(part_bytes(b.pdx, d->M, d->K)) : 0);
+    b.bytes = b.dwp_at + (b.dw ? part_bytes(b.pdw, d->N, d->K) : 0);
     return b;
+}
+
+void set(GemmArgs& a, const Plan& p, void* parts) {
+    a.ti = (uint32_t)p.ti, a.tj = (uint32_t)p.tj, a.splits = p.splits, a.rsplit = p.rsplit, a.part = (float*)parts;
 }
 
 }  // namespace
@@ -134,7 +144,7 @@ extern "C" {
 
 int64_t psfm_linear_fwd_ws_bytes(const psfm_linear* d) {
     if (check(d)) return -1;
-    return part_bytes(plan(d->dtype, d->M, d->N, d->K), d->M, d->N);
+    return skinny(d) ? 0 : part_bytes(plan(d->dtype, d->M, d->N, d->K), d->M, d->N);
 }
 
 int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const void* bias, const void* res, void* y,
@@ -143,12 +153,24 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
     if (d->M == 0 || d->N == 0) return 0;
     if (!y || (d->K > 0 && (!x || !w))) return fail(-9, "psfm_linear_fwd: null tensor");
     if (res && d->ldr < d->N) return fail(-3, "psfm_linear_fwd: ldr below N");
+    const LinearOps& o = ops_of(d->dtype);
+    const hipStream_t s = (hipStream_t)stream;
+    const LinearEpi e{y, bias, res, d->ldr, z, d->act, 1.0f, drop_of(d)};
+    const int64_t v = 16 / size_of(d->dtype);
+    const bool vec = mult(x, d->ldx, d->K, v) && mult(w, d->K, d->K, v);
+    if (skinny(d)) {
+        if (up(d->N, 16) > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more columns than a launch holds");
+        return status(o.skinny(vec, SkinnyArgs{x, w, d->ldx, d->M, d->N, d->K, e}, s), "psfm_linear_fwd: launch");
+    }
     const Plan p = plan(d->dtype, d->M, d->N, d->K);
-    if (part_bytes(p, d->M, d->N) > 0 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
+    if (p.splits > 1 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
+    if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more tiles than a launch holds");
     GemmArgs a{};
-    a.P = x, a.Q = w, a.ldp = d->ldx, a.ldq = d->K, a.I = d->M, a.J = d->N, a.R = d->K;
-    a.e = LinearEpi{y, bias, res, d->ldr, z, d->act, 1.0f, drop_of(d)};
-    return run_gemm(GEMM_FWD, d->dtype, a, p, ws, (hipStream_t)stream);
+    a.P = x, a.Q = w, a.ldp = d->ldx, a.ldq = d->K, a.I = d->M, a.J = d->N, a.R = d->K, a.e = e;
+    set(a, p, ws);
+    int rc = o.forward(p.variant, vec, a, s);
+    if (rc == 0 && p.splits > 1) rc = o.join(a, s);
+    return status(rc, "psfm_linear_fwd: launch");
 }
 
 int64_t psfm_linear_bwd_ws_bytes(const psfm_linear* d, int want_dx, int want_dw, int want_db) {
@@ -164,35 +186,51 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
         return fail(-9, "psfm_linear_bwd: null tensor");
     const BwdPlan b = bwd_plan(d, dx, dw, db);
     if (b.bytes > 0 && !ws) return fail(-10, "psfm_linear_bwd: no workspace");
-    if (b.cols.gx > 0x7fffffff) return fail(-8, "psfm_linear_bwd: more columns than a launch holds");
+    const int64_t most = 0x7fffffff;
+    if (b.cols.gx > most || (b.dx && b.pdx.blocks() > most / 2) || (b.dw && b.pdw.blocks() > most / 2))
+        return fail(-8, "psfm_linear_bwd: more tiles than a launch holds");
     const hipStream_t s = (hipStream_t)stream;
     const LinearOps& o = ops_of(d->dtype);
     const DropArgs drop = drop_of(d);
-    float* cols = (float*)((char*)ws + b.cols_at);
-    const void* dz = b.dz ? ws : dy;
-    if (any && (b.dz || db)) {
-        const DzArgs a{dy, d->act != PSFM_ACT_NONE ? z : nullptr, b.dz ? ws : nullptr, db ? cols : nullptr,
-                       d->M, d->N, b.cols.rows, d->act, drop};
+    const DzArgs make{d->act != PSFM_ACT_NONE ? z : nullptr, d->act, drop, nullptr, nullptr};
+    char* at = (char*)ws;
+    float* cols = (float*)(at + b.cols_at);
+    if (b.pass) {
+        DzPassArgs a{dy, b.dz ? ws : nullptr, d->M, d->N, b.cols.rows, make};
+        a.dz.cols = b.parts ? cols : nullptr;
         if (const int rc = status(o.dz(a, b.cols.gx, b.cols.gy, s), "psfm_linear_bwd: dz launch")) return rc;
     }
-    if (db && d->N > 0) {
-        const int e = o.colsum(cols, any ? b.cols.gy : 0, d->N, drop.scale, db, s);
-        if (const int rc = status(e, "psfm_linear_bwd: column sums launch")) return rc;
-    }
-    void* parts = (char*)ws + b.parts_at;
-    if (dx && d->M > 0 && d->K > 0) {
-        GemmArgs a{};
+    const void* dz = b.dz ? ws : dy;
+    const int64_t v = 16 / size_of(d->dtype);
+    PairArgs pair{};
+    if (b.dx) {
+        GemmArgs& a = pair.dx;
         a.P = dz, a.Q = w, a.ldp = d->N, a.ldq = d->K, a.I = d->M, a.J = d->K, a.R = d->N;
-        a.e.out = dx, a.e.alpha = drop.scale;
-        if (const int rc = run_gemm(GEMM_DX, d->dtype, a, b.dx, parts, s)) return rc;
+        a.e.out = dx, a.e.alpha = drop.scale, a.dz = make;
+        set(a, b.pdx, at + b.dxp_at);
     }
-    if (dw && d->N > 0 && d->K > 0) {
-        GemmArgs a{};
+    if (b.dw) {
+        GemmArgs& a = pair.dw;
         a.P = dz, a.Q = x, a.ldp = d->N, a.ldq = d->ldx, a.I = d->N, a.J = d->K, a.R = d->M;
-        a.e.out = dw, a.e.alpha = drop.scale;
-        if (const int rc = run_gemm(GEMM_DW, d->dtype, a, b.dw, parts, s)) return rc;
+        a.e.out = dw, a.e.alpha = drop.scale, a.dz = make;
+        if (db && !b.pass) (b.parts ? (void*&)a.dz.cols : a.dz.db) = b.parts ? (void*)cols : db;
+        set(a, b.pdw, at + b.dwp_at);
     }
-    return 0;
+    const bool vec = d->N % v == 0 && d->K % v == 0 && ((uintptr_t)dz & 15) == 0 && (!make.z || ((uintptr_t)z & 15) == 0) &&
+                     (!b.dx || ((uintptr_t)w & 15) == 0) && (!b.dw || mult(x, d->ldx, d->K, v));
+    const bool together = b.dx && b.dw && b.pdx.variant == b.pdw.variant;
+    for (int part = 0; part < (together ? 1 : 2); ++part) {
+        pair.ndx = b.dx && part == 0 ? pair.dx.blocks() : 0;
+        pair.ndw = b.dw && (together || part == 1) ? pair.dw.blocks() : 0;
+        if (pair.ndx + pair.ndw == 0) continue;
+        const int rc = o.pair(pair.ndx ? b.pdx.variant : b.pdw.variant, vec, b.stage, pair, s);
+        if (rc) return status(rc, "psfm_linear_bwd: launch");
+    }
+    FinishArgs f{};
+    f.dx = pair.dx, f.dw = pair.dw;
+    // no rows or no products to sum: the bias gradient of no parts is zero
+    if (db && d->N > 0 && (b.parts || !any || !b.stage || !b.dw)) f.cols = cols, f.parts = b.parts, f.N = d->N, f.alpha = drop.scale, f.db = db;
+    return status(o.finish(f, s), "psfm_linear_bwd: finish launch");
 }
 
 const char* psfm_linear_last_error(void) { return g_err.c_str(); }

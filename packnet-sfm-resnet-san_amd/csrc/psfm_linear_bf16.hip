@@ -3,7 +3,7 @@
 
 namespace psfm {
 const LinearOps& linear_ops_bf16() {
-    static const LinearOps ops = {gemm_of<__bf16>, join_of<__bf16>, dz_of<__bf16>, colsum_of<__bf16>};
-    return ops;
+    static const LinearOps o = ops<__bf16>();
+    return o;
 }
 }  // namespace psfm

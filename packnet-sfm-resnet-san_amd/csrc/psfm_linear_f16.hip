@@ -3,7 +3,7 @@
 
 namespace psfm {
 const LinearOps& linear_ops_f16() {
-    static const LinearOps ops = {gemm_of<_Float16>, join_of<_Float16>, dz_of<_Float16>, colsum_of<_Float16>};
-    return ops;
+    static const LinearOps o = ops<_Float16>();
+    return o;
 }
 }  // namespace psfm

@@ -3,7 +3,7 @@
 
 namespace psfm {
 const LinearOps& linear_ops_f32() {
-    static const LinearOps ops = {gemm_of<float>, join_of<float>, dz_of<float>, colsum_of<float>};
-    return ops;
+    static const LinearOps o = ops<float>();
+    return o;
 }
 }  // namespace psfm

@@ -87,9 +87,12 @@ def as_rows(t):
     return t, ld
 
 
-def on_device(t):
-    """Launches go to the current device: make it t's."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_HERE = nullcontext()
+
+
+def on_device(device):
+    """Launches go to the current device: make it this one."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def keep_mask(rows, cols, p, rng):
@@ -123,12 +126,13 @@ def _launch(x, residual, p, rng, share):
     x, ldx = as_rows(x)
     res, ldr = (None, 0) if residual is None else as_rows(residual)
     cols = x.shape[-1]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if y.numel():
-        with on_device(x):
-            _hip.check(_hip.lib().psfm_dropout(_hip.ptr(x), ldx, _hip.ptr(res), ldr, _hip.DTYPES[x.dtype],
-                                               x.numel() // cols, cols, share, p, _hip.ptr(rng), _hip.ptr(y),
-                                               _hip.stream(x.device)), "psfm_dropout")
+    device, dtype, n = x.device, x.dtype, x.numel()
+    y = torch.empty(x.shape, device=device, dtype=dtype)
+    if n:
+        with on_device(device):
+            _hip.check(_hip.lib().psfm_dropout(x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr,
+                                               _hip.DTYPES[dtype], n // cols, cols, share, p, rng.data_ptr(),
+                                               y.data_ptr(), _hip.stream(device)), "psfm_dropout")
     return y
 
 
@@ -208,7 +212,7 @@ class CounterDropout(nn.Module):
             self.state[1] += 1
             return Drop(self.p, used, self.channels)
         used = torch.empty_like(self.state)
-        with on_device(self.state):
+        with on_device(self.state.device):
             _hip.check(_hip.lib().psfm_rng_next(_hip.ptr(self.state), _hip.ptr(used), _hip.stream(self.state.device)),
                        "psfm_rng_next")
         return Drop(self.p, used, self.channels)

@@ -30,33 +30,33 @@ _PLAIN = {ACT_NONE: lambda z: z, ACT_RELU: torch.relu, ACT_SIGMOID: torch.sigmoi
 _Z = {torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
 
 
-def _desc(x, ldx, ldr, N, act, p, rng, share):
-    K = x.shape[-1]
-    M = x.numel() // K if K else x.shape[:-1].numel()
-    return _hip.Linear(M, N, K, ldx, ldr, _hip.DTYPES[x.dtype], act, p, share, None if rng is None else rng.data_ptr())
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _forward(x, weight, bias, residual, act, p, rng, share, want_z):
-    """(x as the kernel took it, weight, y, z)"""
+    """(x as the kernel took it, its row stride, weight, y, z)"""
     x, ldx = as_rows(x)
     weight = weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    residual, ldr = (None, 0) if residual is None else as_rows(residual)
-    N = weight.shape[0]
-    shape = x.shape[:-1] + (N,)
-    d = _desc(x, ldx, ldr, N, act, p, rng, share)
+    if bias is not None:
+        bias = bias.contiguous()
+    ldr = 0
+    if residual is not None:
+        residual, ldr = as_rows(residual)
+    N, K = weight.shape
+    device, dtype, lead = x.device, x.dtype, x.shape[:-1]
+    y = torch.empty(lead + (N,), device=device, dtype=dtype)
+    z = torch.empty(lead + (N,), device=device, dtype=dtype if act == ACT_RELU else _Z[dtype]) if want_z else None
+    d = ctypes.byref(_hip.Linear(lead.numel(), N, K, ldx, ldr, _hip.DTYPES[dtype], act, p, share, _at(rng)))
     L = _hip.lib()
-    y = torch.empty(shape, device=x.device, dtype=x.dtype)
-    z = torch.empty(shape, device=x.device, dtype=x.dtype if act == ACT_RELU else _Z[x.dtype]) if want_z else None
-    n = L.psfm_linear_fwd_ws_bytes(ctypes.byref(d))
+    n = L.psfm_linear_fwd_ws_bytes(d)
     if n < 0:
         _hip.check(-1, "psfm_linear_fwd_ws_bytes")
-    ws = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
-    with on_device(x):
-        _hip.check(L.psfm_linear_fwd(ctypes.byref(d), _hip.ptr(x), _hip.ptr(weight), _hip.ptr(bias),
-                                     _hip.ptr(residual), _hip.ptr(y), _hip.ptr(z), _hip.ptr(ws),
-                                     _hip.stream(x.device)), "psfm_linear_fwd")
-    return x, weight, y, z
+    ws = torch.empty(n, device=device, dtype=torch.uint8) if n else None
+    with on_device(device):
+        _hip.check(L.psfm_linear_fwd(d, x.data_ptr(), weight.data_ptr(), _at(bias), _at(residual), y.data_ptr(), _at(z),
+                                     _at(ws), _hip.stream(device)), "psfm_linear_fwd")
+    return x, ldx, weight, y, z
 
 
 class _LinearAct(torch.autograd.Function):
@@ -68,10 +68,10 @@ class _LinearAct(torch.autograd.Function):
         _hip.note_forward(ctx)
         from_y = act == ACT_RELU and residual is None and rng is None
         want_z = act != ACT_NONE and not from_y and any(ctx.needs_input_grad[:3])
-        xk, wk, y, z = _forward(x, weight, bias, residual, act, p, rng, share, want_z)
-        ctx.save_for_backward(xk if ctx.needs_input_grad[1] else None, wk if ctx.needs_input_grad[0] else None,
-                              y if from_y else z, rng)
-        ctx.meta = (x.shape, wk.shape, None if bias is None else bias.shape, act, p, share)
+        need = ctx.needs_input_grad
+        xk, ldx, wk, y, z = _forward(x, weight, bias, residual, act, p, rng, share, want_z)
+        ctx.save_for_backward(xk if need[1] else None, wk if need[0] else None, y if from_y else z, rng)
+        ctx.meta = (x.shape, ldx, wk.shape, act, p, share)
         return y
 
     @staticmethod
@@ -79,28 +79,28 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, dy):
         _hip.capture_guard(ctx, leaves=True)
         x, weight, z, rng = ctx.saved_tensors
-        xshape, (N, K), bshape, act, p, share = ctx.meta
-        need = ctx.needs_input_grad
-        if not any(need[:3]):
-            return None, None, None, dy, None, None, None, None
-        dyc = dy.contiguous()
-        new = lambda shape: torch.empty(shape, device=dy.device, dtype=dy.dtype)  # noqa: E731
-        dx = new(xshape) if need[0] else None
-        dw = new((N, K)) if need[1] else None
-        db = new(bshape) if need[2] else None
-        M = dy.numel() // N if N else xshape[:-1].numel()
-        d = _hip.Linear(M, N, K, as_rows(x)[1] if x is not None else K, 0, _hip.DTYPES[dy.dtype], act, p, share,
-                        None if rng is None else rng.data_ptr())
-        L = _hip.lib()
-        n = L.psfm_linear_bwd_ws_bytes(ctypes.byref(d), dx is not None, dw is not None, db is not None)
-        if n < 0:
-            _hip.check(-1, "psfm_linear_bwd_ws_bytes")
-        ws = torch.empty(n, device=dy.device, dtype=torch.uint8) if n else None
-        with on_device(dy):
-            _hip.check(L.psfm_linear_bwd(ctypes.byref(d), _hip.ptr(dyc), _hip.ptr(x), _hip.ptr(weight), _hip.ptr(z),
-                                         _hip.ptr(dx), _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws),
-                                         _hip.stream(dy.device)), "psfm_linear_bwd")
-        return dx, dw, db, dy if need[3] else None, None, None, None, None
+        xshape, ldx, (N, K), act, p, share = ctx.meta
+        want_dx, want_dw, want_db, want_dres = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if want_dx or want_dw or want_db:
+            g = dy.contiguous()
+            device, dtype = g.device, g.dtype
+            if want_dx:
+                dx = torch.empty(xshape, device=device, dtype=dtype)
+            if want_dw:
+                dw = torch.empty((N, K), device=device, dtype=dtype)
+            if want_db:
+                db = torch.empty((N,), device=device, dtype=dtype)
+            d = ctypes.byref(_hip.Linear(xshape[:-1].numel(), N, K, ldx, 0, _hip.DTYPES[dtype], act, p, share, _at(rng)))
+            L = _hip.lib()
+            n = L.psfm_linear_bwd_ws_bytes(d, want_dx, want_dw, want_db)
+            if n < 0:
+                _hip.check(-1, "psfm_linear_bwd_ws_bytes")
+            ws = torch.empty(n, device=device, dtype=torch.uint8) if n else None
+            with on_device(device):
+                _hip.check(L.psfm_linear_bwd(d, g.data_ptr(), _at(x), _at(weight), _at(z), _at(dx), _at(dw), _at(db),
+                                             _at(ws), _hip.stream(device)), "psfm_linear_bwd")
+        return dx, dw, db, dy if want_dres else None, None, None, None, None
 
 
 def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):
@@ -133,7 +133,7 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad
                                     or residual is not None and residual.requires_grad):
         return _LinearAct.apply(x, weight, bias, residual, act, p, rng, share)
-    return _forward(x, weight, bias, residual, act, p, rng, share, False)[2]
+    return _forward(x, weight, bias, residual, act, p, rng, share, False)[3]
 
 
 def conv1x1_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):

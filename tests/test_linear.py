@@ -140,7 +140,9 @@ def test_forward_and_gradients(dev, dtype, M, N, K):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_every_subset_of_gradients(dev, dtype):
-    """Only what is asked for is made, and it does not depend on what else is."""
+    """Only what is asked for is made, and it does not depend on what else is: bit for bit, but for the bias
+    gradient, whose rows are summed in another order where no product runs beside it.  Two orders of 70 fp32 terms
+    differ by at most 2 x 72 x 2^-24 of the sum of their magnitudes, and each result is rounded once, eps / 2."""
     t = make(70, 48, 90, dtype, dev, 4, True, True, grad=False)
     drop, _ = drop_and_keep(70, 48, 0.3, dev)
     names, full = ("x", "w", "bias", "res"), None
@@ -154,7 +156,12 @@ def test_every_subset_of_gradients(dev, dtype):
                 full = {**(full or {}), act: got}
             for i, k in enumerate(names):
                 assert (got[k] is None) == (not bits >> i & 1)
-                assert got[k] is None or torch.equal(got[k], full[act][k])
+                if k == "bias" and got[k] is not None:
+                    most = 1.13 / 0.7 * t["dy"].double().abs().sum(0)
+                    step = torch.finfo(dtype).eps * full[act][k].double().abs()
+                    assert bool(((got[k].double() - full[act][k].double()).abs() <= 144 * U * most + 1.01 * step).all())
+                else:
+                    assert got[k] is None or torch.equal(got[k], full[act][k])
 
 
 @gpu
