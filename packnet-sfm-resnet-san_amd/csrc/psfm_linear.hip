@@ -58,13 +58,17 @@ struct Plan {
     int64_t blocks() const { return ti * tj * splits; }
 };
 
-// Tiles: the largest that still fills the 256 CUs, else the smallest.  The reduction is split while the tiles alone
-// leave CUs idle and a split keeps at least four LDS stages.
-Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int variant = -1) {
+// Tiles: the largest that still fills the 256 CUs and computes at most an eighth more than the smallest
+// would (a 64-column layer in 256-column tiles: 86 us, 42 in 128), else the smallest.  The reduction is split while
+// the tiles alone leave CUs idle and a split keeps at least four LDS stages.
+Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1) {
     Plan p{0, 0, 0, 0, 1};
-    for (int v = variant >= 0 ? variant : dtype == PSFM_DTYPE_F32 ? 1 : 2; v >= 0; --v) {
-        p.variant = v, p.ti = up(I, LINEAR_TILES[v].bi), p.tj = up(J, LINEAR_TILES[v].bj);
-        if (p.ti * p.tj >= 256 || v == variant) break;
+    const Tile& t0 = LINEAR_TILES[0];
+    const double least = (double)(up(I, t0.bi) * t0.bi) * (double)(up(J, t0.bj) * t0.bj);
+    for (int v = std::min(largest, dtype == PSFM_DTYPE_F32 ? 1 : 2); v >= 0; --v) {
+        const Tile& t = LINEAR_TILES[v];
+        p.variant = v, p.ti = up(I, t.bi), p.tj = up(J, t.bj);
+        if (p.ti * p.tj >= 256 && (double)(p.ti * t.bi) * (double)(p.tj * t.bj) <= 1.125 * least) break;
     }
     const int64_t stage = 128 / size_of(dtype), stages = up(R, stage), tiles = p.ti * p.tj;
     int64_t splits = 1;
@@ -109,19 +113,19 @@ struct BwdPlan {
 };
 
 // The products share a launch where they share a tile.  They make dz themselves where that repeats little: every tile
-// column of either makes it once, and a pass of its own costs a launch and dz's way to memory and back.
+// column of either makes it once, in the smallest tiles, and a pass of its own costs a launch and dz's way to
+// memory and back.
 BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db) {
     BwdPlan b{};
     const bool any = d->M > 0 && d->N > 0, make = d->act != PSFM_ACT_NONE || drop_of(d).rng;
     b.dx = want_dx && d->M > 0 && d->K > 0;
     b.dw = want_dw && d->N > 0 && d->K > 0;
-    if (b.dx) b.pdx = plan(d->dtype, d->M, d->K, d->N);
-    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M);
-    // at the largest tile the instances that make dz are not built: their columns are many
-    const int64_t columns = (b.dx ? b.pdx.tj : 0) + (b.dw ? b.pdw.tj : 0);
-    const bool large = (b.dx && b.pdx.variant > 1) || (b.dw && b.pdw.variant > 1);
+    const int64_t columns = (b.dx + b.dw) * up(d->K, LINEAR_TILES[0].bj);
     const bool cheap = columns <= 4 || (double)columns * (double)d->M * (double)d->N < 8e6;
-    b.stage = any && (b.dx || b.dw) && !large && cheap && (make || (want_db && b.dw));
+    b.stage = any && (b.dx || b.dw) && cheap && (make || (want_db && b.dw));
+    const int largest = b.stage ? 0 : LINEAR_NTILES - 1;
+    if (b.dx) b.pdx = plan(d->dtype, d->M, d->K, d->N, largest);
+    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M, largest);
     b.pass = any && !b.stage && ((make && (b.dx || b.dw)) || want_db);
     if (b.stage && want_db && !b.dw) b.pass = true;      // the column sums alone
     b.dz = b.pass && !b.stage && make && (b.dx || b.dw);

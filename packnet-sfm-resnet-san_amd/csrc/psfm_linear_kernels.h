@@ -23,6 +23,10 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
+// LDS by its own address space: the compiler follows such pointers to their object (the waits for loads into it)
+#define PSFM_LDS __attribute__((address_space(3)))
+typedef PSFM_LDS uint8_t lds8;
+
 template <typename T>
 constexpr int CHUNK = 16 / (int)sizeof(T);   // values of one 16-byte chunk
 
@@ -241,15 +245,53 @@ struct Stager {
             r[q] = load_n<T, VEC>(base + (n > 0 ? row * ld + col : 0), n);
         }
     }
-    static __device__ __forceinline__ void put(uint8_t* lds, int q, u4v v) {
+    static __device__ __forceinline__ void put(lds8* lds, int q, u4v v) {
         const int c = q * NTH + threadIdx.x;
         const int row = TURNED ? c / CPR : c / 8, ch = TURNED ? c % CPR : c % 8;
         const int x = TURNED ? swz_turned<T, B>(row) : swz_straight(row);
-        *reinterpret_cast<u4v*>(lds + row * (TURNED ? CPR * 16 : 128) + ((ch ^ x) << 4)) = v;
+        *(PSFM_LDS u4v*)(lds + row * (TURNED ? CPR * 16 : 128) + ((ch ^ x) << 4)) = v;
     }
-    __device__ __forceinline__ void store(uint8_t* lds) const {
+    __device__ __forceinline__ void store(lds8* lds) const {
 #pragma unroll
         for (int q = 0; q < NC; ++q) put(lds, q, r[q]);
+    }
+};
+
+// The same without registers: the loads write LDS themselves, 16 bytes a lane in lane order, so the chunks' order in
+// a row is turned in the addresses that they read.  Whole chunks only.  A row or column that does not exist reads
+// the last one that does (what it gives is never stored); behind the reduction's end there are zeros.
+__device__ const uint4 zeros16 = {0, 0, 0, 0};
+
+template <typename T, int B, int NTH, bool TURNED>
+struct DmaStager {
+    static constexpr int NC = B * 8 / NTH, V = CHUNK<T>, CPR = B * (int)sizeof(T) / 16, BR = 128 / (int)sizeof(T);
+    const T* p[NC];       // this lane's chunks of the next stage
+    int r[NC];            // their reduction index in the stage
+    int64_t stride;       // from stage to stage
+
+    __device__ __forceinline__ void at(const T* base, int64_t ld, int64_t b0, int64_t ext, int64_t r0) {
+        stride = TURNED ? BR * ld : BR;
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const int c = q * NTH + threadIdx.x, row = TURNED ? c / CPR : c / 8;
+            const int ch = TURNED ? (c % CPR) ^ swz_turned<T, B>(row) : (c % 8) ^ swz_straight(row);
+            const int64_t want = b0 + (TURNED ? ch * V : row), last = TURNED ? ext - V : ext - 1;
+            const int64_t out = want < last ? want : last;
+            r[q] = TURNED ? row : ch * V;
+            p[q] = base + (TURNED ? (r0 + row) * ld + out : out * ld + r0 + ch * V);
+        }
+    }
+    // left: reduction elements from this stage on
+    __device__ __forceinline__ void load(lds8* lds, int64_t left) {
+        typedef __attribute__((address_space(1))) const void gvoid;
+        typedef PSFM_LDS void lvoid;
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const T* src = p[q];
+            if (left < BR && r[q] >= left) src = (const T*)&zeros16;
+            __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(lds + (q * NTH + (threadIdx.x & ~63)) * 16), 16, 0, 0);
+            p[q] += stride;
+        }
     }
 };
 
@@ -285,7 +327,7 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
             }
         }
     }
-    __device__ __forceinline__ void store(uint8_t* lds, const GemmArgs& A, const PhiloxKey& key, int64_t b0, int64_t r0) {
+    __device__ __forceinline__ void store(lds8* lds, const GemmArgs& A, const PhiloxKey& key, int64_t b0, int64_t r0) {
         typedef T TV __attribute__((ext_vector_type(V)));
 #pragma unroll
         for (int q = 0; q < S::NC; ++q) {
@@ -329,11 +371,11 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
 // One lane's operand of a matrix instruction step (64 bytes of reduction: 32 values of 16 bits, 16 of 32): the 16
 // output rows or columns b .. b + 15, lane l holds row l % 16, reduction chunk l / 16.
 template <typename T, int B, bool TURNED>
-__device__ __forceinline__ u4v fragment(const uint8_t* lds, int b, int ks) {
+__device__ __forceinline__ u4v fragment(const lds8* lds, int b, int ks) {
     const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
     if (!TURNED) {
         const int row = b + n;
-        return *reinterpret_cast<const u4v*>(lds + row * 128 + (((ks * 4 + g) ^ swz_straight(row)) << 4));
+        return *(const PSFM_LDS u4v*)(lds + row * 128 + (((ks * 4 + g) ^ swz_straight(row)) << 4));
     }
     constexpr int RB = B * (int)sizeof(T);
     if constexpr (sizeof(T) == 4) {
@@ -341,12 +383,12 @@ __device__ __forceinline__ u4v fragment(const uint8_t* lds, int b, int ks) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = ks * 16 + 4 * g + i, ch = (b >> 2) + (n >> 2);
-            v[i] = *reinterpret_cast<const uint32_t*>(lds + row * RB + ((ch ^ swz_turned<T, B>(row)) << 4) + 4 * (n & 3));
+            v[i] = *(const PSFM_LDS uint32_t*)(lds + row * RB + ((ch ^ swz_turned<T, B>(row)) << 4) + 4 * (n & 3));
         }
         return v;
     } else {
         // a 16-lane group reads 4 rows x 16 values, lane n gets column n of the 4 rows
-        typedef __attribute__((address_space(3))) s4 lds_s4;
+        typedef PSFM_LDS s4 lds_s4;
         const int ch = (b >> 3) + ((n & 3) >> 1), r0 = ks * 32 + 8 * g + (n >> 2), r1 = r0 + 4;
         const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (lds_s4*)(lds + r0 * RB + ((ch ^ swz_turned<T, B>(r0)) << 4) + 8 * (n & 1)));
@@ -354,6 +396,59 @@ __device__ __forceinline__ u4v fragment(const uint8_t* lds, int b, int ks) {
             (lds_s4*)(lds + r1 * RB + ((ch ^ swz_turned<T, B>(r1)) << 4) + 8 * (n & 1)));
         typedef short s8 __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(u4v, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    }
+}
+
+// S of them of a turned 16-bit operand, 16 output rows apart, where the stages are filled by loads into LDS: behind such
+// a load the compiler puts a wait for all of them before the first transposing read (it does not follow the object
+// that this read reads, as it does for plain reads), so the reads are written out with their own wait.
+// One address serves all: the operands' chunks differ in bits that the swizzle XORs (s << 5), the rows of the second half
+// and of the second step lie a constant away and are swizzled alike.  It is hidden from the optimiser each
+// time, which would keep every operand's own and spill.
+template <int S, int B, int ks>
+__device__ __forceinline__ void fragments_turned(const lds8* lds, int b, u4v (&f)[S]) {
+    constexpr int RB = B * 2, U = S % 4 == 0 ? 4 : 2;
+    static_assert(S % 2 == 0 && S * 2 <= B / 8, "operands within a row");
+    const int l = threadIdx.x & 63, g = l >> 4, n = l & 15, row = 8 * g + (n >> 2), ch = (b >> 3) + ((n & 3) >> 1);
+    typedef unsigned int u2v __attribute__((ext_vector_type(2)));
+    uint32_t at = (uint32_t)(uintptr_t)(lds + row * RB + ((ch ^ swz_turned<__bf16, B>(row)) << 4) + 8 * (n & 1));
+    asm volatile("" : "+v"(at));
+    constexpr int o0 = ks * 32 * RB, o1 = o0 + 4 * RB;
+#pragma unroll
+    for (int s = 0; s < S; s += U) {
+        u2v v[2 * U];
+        if constexpr (U == 4)
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                : "v"(at ^ s << 5), "v"(at ^ (s + 1) << 5), "v"(at ^ (s + 2) << 5), "v"(at ^ (s + 3) << 5), "n"(o0),
+                  "n"(o1)
+                : "memory");
+        else
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                : "v"(at ^ s << 5), "v"(at ^ (s + 1) << 5), "n"(o0), "n"(o1)
+                : "memory");
+#pragma unroll
+        for (int q = 0; q < U; ++q) f[s + q] = u4v{v[2 * q][0], v[2 * q][1], v[2 * q + 1][0], v[2 * q + 1][1]};
+    }
+}
+
+// The S operands of a wave's step.
+template <typename T, int S, int B, bool TURNED, bool DMA, int ks>
+__device__ __forceinline__ void fragments(const lds8* lds, int b, u4v (&f)[S]) {
+    if constexpr (TURNED && DMA && sizeof(T) == 2) {
+        fragments_turned<S, B, ks>(lds, b, f);
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s) f[s] = fragment<T, B, TURNED>(lds, b + 16 * s, ks);
     }
 }
 
@@ -378,11 +473,13 @@ __device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
     return x * per + (x < more ? x : more) + k;
 }
 
-// Tile `id` of `count` of a product.  WI x WJ waves.
+// Tile `id` of `count` of a product.  WI x WJ waves.  The two stages are two objects, and the loop is written out for
+// both, so that the compiler sees that the reads of one do not wait for the loads into the other.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, bool VEC, bool FULL, bool DZ>
 __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t count,
-                                        uint8_t (&smem)[2][(BI + BJ) * 128]) {
+                                        uint8_t (&stage0)[(BI + BJ) * 128], uint8_t (&stage1)[(BI + BJ) * 128]) {
     constexpr int NTH = 64 * WI * WJ, BR = 128 / (int)sizeof(T), SI = BI / WI / 16, SJ = BJ / WJ / 16, V = CHUNK<T>;
+    constexpr bool DMA = VEC && !DZ;
     const uint32_t tiles = A.ti * A.tj, w = xcd_run(id, count), split = w / tiles, t = w - split * tiles;
     const uint32_t band = t / (8 * A.tj), in = t - band * 8 * A.tj, high = A.ti - band * 8 < 8 ? A.ti - band * 8 : 8;
     const int64_t i0 = (int64_t)(band * 8 + in % high) * BI, j0 = (int64_t)(in / high) * BJ;
@@ -395,62 +492,88 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     for (int a = 0; a < SI; ++a)
 #pragma unroll
         for (int b = 0; b < SJ; ++b) acc[a][b] = f4{0, 0, 0, 0};
-    std::conditional_t<DZ, DzStager<T, BI, NTH, PT, VEC>, Stager<T, BI, NTH, PT, VEC>> sp;
-    Stager<T, BJ, NTH, QT, VEC> sq;
+    using SP = std::conditional_t<DZ, DzStager<T, BI, NTH, PT, VEC>,
+                                  std::conditional_t<DMA, DmaStager<T, BI, NTH, PT>, Stager<T, BI, NTH, PT, VEC>>>;
+    using SQ = std::conditional_t<DMA, DmaStager<T, BJ, NTH, QT>, Stager<T, BJ, NTH, QT, VEC>>;
+    SP sp;
+    SQ sq;
+    const T* P = (const T*)A.P;
+    const T* Q = (const T*)A.Q;
     PhiloxKey dkey{};
     if constexpr (DZ) {
         if (A.dz.drop.rng) dkey = philox_key(A.dz.drop.rng);
 #pragma unroll
         for (int k = 0; k < V; ++k) sp.sum[k] = 0;
     }
-    const T* P = (const T*)A.P;
-    const T* Q = (const T*)A.Q;
-    auto fetch = [&](int64_t r) {
-        if constexpr (DZ)
-            sp.load(A, i0, A.I, r, rend);
-        else
-            sp.load(P, A.ldp, i0, A.I, r, rend);
-        sq.load(Q, A.ldq, j0, A.J, r, rend);
-    };
-    auto stage = [&](uint8_t* lds, int64_t r) {
-        if constexpr (DZ)
-            sp.store(lds, A, dkey, i0, r);
-        else
-            sp.store(lds);
-        sq.store(lds + BI * 128);
-    };
-    if (nk > 0) {
-        fetch(r0);
-        stage(smem[0], r0);
+    if constexpr (DMA) {
+        sp.at(P, A.ldp, i0, A.I, r0);
+        sq.at(Q, A.ldq, j0, A.J, r0);
     }
-    __syncthreads();
-    for (int k = 0; k < nk; ++k) {
-        const bool more = k + 1 < nk;
-        const int64_t next = r0 + (int64_t)(k + 1) * BR;
-        if (more) fetch(next);
-        const uint8_t* lp = smem[k & 1];
-        const uint8_t* lq = lp + BI * 128;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            u4v fp[SI], fq[SJ];
-#pragma unroll
-            for (int a = 0; a < SI; ++a) fp[a] = fragment<T, BI, PT>(lp, wi * (BI / WI) + a * 16, ks);
-#pragma unroll
-            for (int b = 0; b < SJ; ++b) fq[b] = fragment<T, BJ, QT>(lq, wj * (BJ / WJ) + b * 16, ks);
-#pragma unroll
-            for (int a = 0; a < SI; ++a)
-#pragma unroll
-                for (int b = 0; b < SJ; ++b) acc[a][b] = mma<T>(fq[b], fp[a], acc[a][b]);
+    // the stage at reduction r: its loads go out, into LDS or registers; what came to registers is put to LDS
+    auto fetch = [&](lds8* lds, int64_t r) {
+        if constexpr (DMA) {
+            sp.load(lds, rend - r);
+            sq.load(lds + BI * 128, rend - r);
+        } else {
+            if constexpr (DZ)
+                sp.load(A, i0, A.I, r, rend);
+            else
+                sp.load(P, A.ldp, i0, A.I, r, rend);
+            sq.load(Q, A.ldq, j0, A.J, r, rend);
         }
-        if (more) stage(smem[(k + 1) & 1], next);   // its last readers passed the barrier before this step
+    };
+    auto put = [&](lds8* lds, int64_t r) {
+        if constexpr (!DMA) {
+            if constexpr (DZ)
+                sp.store(lds, A, dkey, i0, r);
+            else
+                sp.store(lds);
+            sq.store(lds + BI * 128);
+        }
+    };
+    auto ready = [&]() {   // this wave's loads into LDS have landed, and so have the others' behind the barrier
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+    };
+    auto multiply_step = [&](const lds8* lp, auto ks) {
+        u4v fp[SI], fq[SJ];
+        fragments<T, SJ, BJ, QT, DMA, ks.value>(lp + BI * 128, wj * (BJ / WJ), fq);
+        fragments<T, SI, BI, PT, DMA, ks.value>(lp, wi * (BI / WI), fp);
+#pragma unroll
+        for (int a = 0; a < SI; ++a)
+#pragma unroll
+            for (int b = 0; b < SJ; ++b) acc[a][b] = mma<T>(fq[b], fp[a], acc[a][b]);
+    };
+    auto multiply = [&](const lds8* lp) {
+        multiply_step(lp, std::integral_constant<int, 0>());
+        multiply_step(lp, std::integral_constant<int, 1>());
+    };
+    // the stage that is filled: its last readers passed the barrier before this step
+    auto step = [&](const lds8* now, lds8* next, int k) {
+        const bool more = k + 1 < nk;
+        const int64_t r = r0 + (int64_t)(k + 1) * BR;
+        if (more) fetch(next, r);
+        multiply(now);
+        if (more) put(next, r);
+        ready();
+    };
+    lds8* const s0 = (lds8*)&stage0[0];
+    lds8* const s1 = (lds8*)&stage1[0];
+    if (nk > 0) {
+        fetch(s0, r0);
+        put(s0, r0);
+    }
+    ready();
+    for (int k = 0; k < nk; k += 2) {
+        step(s0, s1, k);
+        if (k + 1 < nk) step(s1, s0, k + 1);
     }
 
     if constexpr (DZ && PT) {
         if (j0 == 0 && (A.dz.cols || A.dz.db)) {   // the bias gradient: this tile's columns, over this split's rows
             constexpr int CPR = BI / V, RP = NTH / CPR;
-            static_assert(RP * BI * 4 <= (int)sizeof(smem), "column sums");
-            float* sums = reinterpret_cast<float*>(&smem[0][0]);
+            static_assert(RP * BI * 4 <= (int)sizeof(stage0), "column sums");
+            float* sums = reinterpret_cast<float*>(&stage0[0]);
 #pragma unroll
             for (int k = 0; k < V; ++k) sums[threadIdx.x / CPR * BI + threadIdx.x % CPR * V + k] = sp.sum[k];
             __syncthreads();
@@ -485,27 +608,27 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     // The epilogue reads the tile back from LDS, 16 bytes of output a thread and whole row segments a wave, in a
     // short loop: unrolled over the accumulators it was 64 copies of the activations and generators, and the
     // instruction fetch took four times the product (silu at 4096 x 8192 x 2048: 884 us, 185 without it).
-    // 16-byte chunks are XORed by the row: the 16 rows of a store hit 16 bank quads.  A tile larger
-    // than the stages goes through in bands of the waves' rows.
-    constexpr int BANDS = BI * BJ * 4 <= (int)sizeof(smem) ? 1 : WI, BAND = BI / BANDS;
+    // 16-byte chunks are XORed by the row: the 16 rows of a store hit 16 bank quads.  The tile goes through the
+    // first stage in bands of rows.
+    constexpr int BANDS = (BI * BJ * 4 + (int)sizeof(stage0) - 1) / (int)sizeof(stage0), BAND = BI / BANDS;
     constexpr int CPR = BJ / V, RPP = NTH / CPR;
-    static_assert(BAND * BJ * 4 <= (int)sizeof(smem) && NTH % CPR == 0 && BAND % RPP == 0, "epilogue tile");
-    float* tile = reinterpret_cast<float*>(&smem[0][0]);
+    static_assert(BI % BANDS == 0 && BAND % 16 == 0 && BAND * BJ * 4 <= (int)sizeof(stage0) && NTH % CPR == 0 &&
+                      BAND % RPP == 0, "epilogue tile");
+    float* tile = reinterpret_cast<float*>(&stage0[0]);
     PhiloxKey key{};
     if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
     const int col = threadIdx.x % CPR * V;
 #pragma unroll
     for (int band = 0; band < BANDS; ++band) {
         if (band) __syncthreads();
-        if (BANDS == 1 || wi == band) {
 #pragma unroll
-            for (int a = 0; a < SI; ++a) {
-                const int i = (BANDS == 1 ? wi * (BI / WI) : 0) + a * 16 + n;
+        for (int a = 0; a < SI; ++a) {
+            const int first = wi * (BI / WI) + a * 16 - band * BAND;
+            if (first < 0 || first >= BAND) continue;
 #pragma unroll
-                for (int b = 0; b < SJ; ++b) {
-                    const int c = (wj * (BJ / WJ) + b * 16) / 4 + g;
-                    *reinterpret_cast<f4*>(tile + i * BJ + ((c ^ (i & 15)) << 2)) = acc[a][b];
-                }
+            for (int b = 0; b < SJ; ++b) {
+                const int c = (wj * (BJ / WJ) + b * 16) / 4 + g;
+                *reinterpret_cast<f4*>(tile + (first + n) * BJ + ((c ^ n) << 2)) = acc[a][b];
             }
         }
         __syncthreads();
@@ -527,27 +650,27 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool VEC>
-__global__ __launch_bounds__(64 * WI * WJ) void k_forward(const GemmArgs A) {
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2][(BI + BJ) * 128];
-    product<T, BI, BJ, WI, WJ, false, false, VEC, true, false>(A, blockIdx.x, gridDim.x, smem);
+__global__ __launch_bounds__(64 * WI * WJ, 2) void k_forward(const GemmArgs A) {
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128];
+    product<T, BI, BJ, WI, WJ, false, false, VEC, true, false>(A, blockIdx.x, gridDim.x, stage0, stage1);
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DZ>
-__global__ __launch_bounds__(64 * WI * WJ) void k_pair(const PairArgs A) {
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2][(BI + BJ) * 128];
+__global__ __launch_bounds__(64 * WI * WJ, 2) void k_pair(const PairArgs A) {
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128];
     if (blockIdx.x < A.ndx)
-        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ>(A.dx, blockIdx.x, A.ndx, smem);
+        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ>(A.dx, blockIdx.x, A.ndx, stage0, stage1);
     else
-        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ>(A.dw, blockIdx.x - A.ndx, A.ndw, smem);
+        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ>(A.dw, blockIdx.x - A.ndx, A.ndw, stage0, stage1);
 }
 
-// y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction; each reads 16 rows of W straight into
-// the matrix instructions' operands, four steps (256 bytes a row) at a time, and x's few rows from the caches.
+// y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction, 64 bytes of each row a step; each reads
+// 16 rows of W straight into the matrix instructions' operands, U steps in flight, and x's few rows from the caches.
 constexpr int SKINNY_WAVES = 8;
 
 template <typename T, int MT, bool VEC>
 __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A) {
-    constexpr int V = CHUNK<T>, STEP = 4 * V, U = 4;
+    constexpr int V = CHUNK<T>, STEP = 4 * V, U = 8 / MT;
     __shared__ f4 part[SKINNY_WAVES][MT][64];
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4, n = l & 15;
     const int64_t j0 = (int64_t)blockIdx.x * 16, j = j0 + n;
@@ -555,11 +678,11 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
     f4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = f4{0, 0, 0, 0};
-    for (int64_t k0 = (int64_t)wave * U * STEP; k0 < A.K; k0 += SKINNY_WAVES * U * STEP) {
+    for (int64_t k0 = (int64_t)wave * STEP; k0 < A.K; k0 += SKINNY_WAVES * U * STEP) {
         u4v fw[U], fx[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t k = k0 + u * STEP + g * V, left = A.K - k;
+            const int64_t k = k0 + u * SKINNY_WAVES * STEP + g * V, left = A.K - k;
             const int have = left >= V ? V : left > 0 ? (int)left : 0;
             fw[u] = load_n<T, VEC>(w + (have ? k : 0), j < A.N ? have : 0);
 #pragma unroll
@@ -738,28 +861,25 @@ int forward_of(int variant, bool vec, const GemmArgs& a, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ>
-void launch_pair(bool vec, bool dz, const PairArgs& a, hipStream_t s) {
+template <typename T, int BI, int BJ, int WI, int WJ, bool DZ>
+void launch_pair(bool vec, const PairArgs& a, hipStream_t s) {
     const dim3 grid(a.ndx + a.ndw), block(64 * WI * WJ);
     if (vec)
-        dz ? k_pair<T, BI, BJ, WI, WJ, true, true><<<grid, block, 0, s>>>(a)
-           : k_pair<T, BI, BJ, WI, WJ, true, false><<<grid, block, 0, s>>>(a);
+        k_pair<T, BI, BJ, WI, WJ, true, DZ><<<grid, block, 0, s>>>(a);
     else
-        dz ? k_pair<T, BI, BJ, WI, WJ, false, true><<<grid, block, 0, s>>>(a)
-           : k_pair<T, BI, BJ, WI, WJ, false, false><<<grid, block, 0, s>>>(a);
+        k_pair<T, BI, BJ, WI, WJ, false, DZ><<<grid, block, 0, s>>>(a);
 }
+// dz is made on the way only in the smallest tiles: the others have no registers left for it
 template <typename T>
 int pair_of(int variant, bool vec, bool dz, const PairArgs& a, hipStream_t s) {
-    if (variant == 0) {
-        launch_pair<T, 64, 64, 2, 2>(vec, dz, a, s);
-    } else if (variant == 1 || sizeof(T) == 4) {
-        launch_pair<T, 128, 128, 2, 2>(vec, dz, a, s);
-    } else if constexpr (sizeof(T) == 2) {   // dz is a pass of its own at this size
-        if (vec)
-            k_pair<T, 256, 256, 2, 4, true, false><<<dim3(a.ndx + a.ndw), 512, 0, s>>>(a);
-        else
-            k_pair<T, 256, 256, 2, 4, false, false><<<dim3(a.ndx + a.ndw), 512, 0, s>>>(a);
-    }
+    if (variant == 0 && dz)
+        launch_pair<T, 64, 64, 2, 2, true>(vec, a, s);
+    else if (variant == 0)
+        launch_pair<T, 64, 64, 2, 2, false>(vec, a, s);
+    else if (variant == 1 || sizeof(T) == 4)
+        launch_pair<T, 128, 128, 2, 2, false>(vec, a, s);
+    else if constexpr (sizeof(T) == 2)
+        launch_pair<T, 256, 256, 2, 4, false>(vec, a, s);
     return (int)hipGetLastError();
 }
 
