@@ -37,9 +37,10 @@ extern "C" {
 int psfm_dropout(const void* x, int64_t ldx, const void* res, int64_t ldr, int dtype, int64_t rows, int64_t cols,
                  int64_t mask_rows, double p, const int64_t* rng, void* y, void* stream);
 
-/* used = state; state.offset += 1 (both int64 [2] on the device): one mask's (seed, offset), drawn in
- * stream order, so that every replay of a captured graph draws the next. */
-int psfm_rng_next(int64_t* state, int64_t* used, void* stream);
+/* used = (state.seed + add, state.offset); state.offset += 1 (both int64 [2] on the device, wrapping): one mask's
+ * (seed, offset), drawn in stream order, so that every replay of a captured graph draws the next.  `add`: the
+ * rank of a data-parallel job, whose ranks hold the same state. */
+int psfm_rng_next(int64_t* state, int64_t add, int64_t* used, void* stream);
 
 const char* psfm_dropout_last_error(void);
 

@@ -196,7 +196,7 @@ def lib():
         # include/psfm_dropout.h
         "psfm_dropout": ([V, ctypes.c_int64, V, ctypes.c_int64, c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                           ctypes.c_double, V, V, V], c_int),
-        "psfm_rng_next": ([V, V, V], c_int),
+        "psfm_rng_next": ([V, ctypes.c_int64, V, V], c_int),
         "psfm_dropout_last_error": ([], ctypes.c_char_p),
         # include/psfm_linear.h
         "psfm_linear_fwd_ws_bytes": ([ctypes.POINTER(Linear)], ctypes.c_int64),

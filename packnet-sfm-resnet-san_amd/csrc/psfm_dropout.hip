@@ -38,7 +38,7 @@ struct Args {
 
 constexpr int UNROLL = 4, THREADS = 256;
 
-template <typename T, bool RES>
+template <typename T, bool RES, bool SHARED>
 __global__ __launch_bounds__(THREADS) void k_dropout(const Args A) {
     constexpr int V = 16 / (int)sizeof(T);
     typedef T TV __attribute__((ext_vector_type(V)));
@@ -67,22 +67,20 @@ __global__ __launch_bounds__(THREADS) void k_dropout(const Args A) {
             }
         }
     }
+    KeepBits<V> keep;   // SHARED: a mask by channel
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         if (row[u] >= A.rows) return;
         TV y;
-        const uint64_t block = A.drop.rng ? mask_block(mask_row(A.drop, row[u]), A.cols, col[u]) : 0;
+        float v[V];
 #pragma unroll
-        for (int q = 0; q < V / 4; ++q) {
-            uint32_t w[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (A.drop.rng) philox4(key, block + q, w);
+        for (int k = 0; k < V; ++k) v[k] = (float)x[u][k];
+        if (SHARED)
+            drop_run(A.drop, key, keep, A.cols, mask_row(A.drop, row[u]), col[u], A.drop.scale, v);
+        else if (A.drop.rng)
+            drop_block(A.drop, key, mask_block(row[u], A.cols, col[u]), A.drop.scale, v);
 #pragma unroll
-            for (int k = 4 * q; k < 4 * q + 4; ++k) {
-                float v = (float)x[u][k];
-                if (A.drop.rng) v = w[k & 3] <= A.drop.last ? 0.0f : v * A.drop.scale;
-                y[k] = (T)(RES ? v + (float)res[u][k] : v);
-            }
-        }
+        for (int k = 0; k < V; ++k) y[k] = (T)(RES ? v[k] + (float)res[u][k] : v[k]);
         T* p = (T*)A.y + row[u] * A.cols + col[u];
         if (col[u] + V <= A.cols) {
             __builtin_memcpy(p, &y, 16);
@@ -99,18 +97,19 @@ int run(const Args& a, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T), PER = THREADS * UNROLL;
     const int64_t blocks = (a.rows * ((a.cols + V - 1) / V) + PER - 1) / PER;
     if (blocks > 0x7fffffff) return fail(-1, "psfm_dropout: more values than a launch holds");
-    if (a.res)
-        k_dropout<T, true><<<dim3((unsigned)blocks), THREADS, 0, s>>>(a);
+    const dim3 grid((unsigned)blocks);
+    if (a.drop.rng && a.drop.mask_rows > 1)
+        a.res ? k_dropout<T, true, true><<<grid, THREADS, 0, s>>>(a) : k_dropout<T, false, true><<<grid, THREADS, 0, s>>>(a);
     else
-        k_dropout<T, false><<<dim3((unsigned)blocks), THREADS, 0, s>>>(a);
+        a.res ? k_dropout<T, true, false><<<grid, THREADS, 0, s>>>(a) : k_dropout<T, false, false><<<grid, THREADS, 0, s>>>(a);
     return status("psfm_dropout: launch");
 }
 
-__global__ void k_rng_next(int64_t* state, int64_t* used) {
-    const int64_t seed = state[0], off = state[1];
-    used[0] = seed;
-    used[1] = off;
-    state[1] = (int64_t)((uint64_t)off + 1);
+__global__ void k_rng_next(int64_t* state, uint64_t add, int64_t* used) {
+    const uint64_t seed = (uint64_t)state[0] + add, off = (uint64_t)state[1];
+    used[0] = (int64_t)seed;
+    used[1] = (int64_t)off;
+    state[1] = (int64_t)(off + 1);
 }
 
 }  // namespace
@@ -135,9 +134,9 @@ int psfm_dropout(const void* x, int64_t ldx, const void* res, int64_t ldr, int d
     return dtype == PSFM_DTYPE_F32 ? run<float>(a, s) : dtype == PSFM_DTYPE_F16 ? run<_Float16>(a, s) : run<__bf16>(a, s);
 }
 
-int psfm_rng_next(int64_t* state, int64_t* used, void* stream) {
+int psfm_rng_next(int64_t* state, int64_t add, int64_t* used, void* stream) {
     if (!state || !used) return fail(-1, "psfm_rng_next: null pointer");
-    k_rng_next<<<1, 1, 0, (hipStream_t)stream>>>(state, used);
+    k_rng_next<<<1, 1, 0, (hipStream_t)stream>>>(state, (uint64_t)add, used);
     return status("psfm_rng_next: launch");
 }
 

@@ -54,7 +54,7 @@ struct SkinnyArgs {
     LinearEpi e;
 };
 
-// Both gradients' products in one launch: workgroups 0 .. dx.blocks() - 1 make dx, the rest dw.
+// Both gradients' products in one launch: workgroups 0 .. ndw - 1 make dw (long reductions first), the rest dx.
 struct PairArgs {
     GemmArgs dx, dw;
     uint32_t ndx, ndw;

@@ -31,9 +31,27 @@ template <typename T>
 constexpr int CHUNK = 16 / (int)sizeof(T);   // values of one 16-byte chunk
 
 // ---- activations, in fp32, of N values under one (uniform) choice ------------------------------
-__device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + __expf(-z)); }
+// v_rcp_f32 is good to one step of fp32, the IEEE division around it costs ten instructions
+__device__ __forceinline__ float sigmoidf(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-template <int N>
+// The normal distribution function and exp(-z^2 / 2).  fp32: erff.  16 bits: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2),
+// t = 1 / (1 + p x), x >= 0 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: 1.5e-7 of error), which
+// shares its exponential with the density and keeps the lower tail's own scale; erff's two branches took
+// a third of the epilogue.
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    e = __expf(-0.5f * z * z);
+    if constexpr (sizeof(T) == 4) {
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    } else {
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678118654752f * fabsf(z));
+        const float q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float low = 0.5f * q * e;
+        return z < 0.0f ? low : 1.0f - low;
+    }
+}
+
+template <typename T, int N>
 __device__ __forceinline__ void act_of(int act, float (&z)[N]) {
 #define PSFM_EACH(F)                         \
     _Pragma("unroll") for (int k = 0; k < N; ++k) { \
@@ -41,12 +59,13 @@ __device__ __forceinline__ void act_of(int act, float (&z)[N]) {
         z[k] = F;                            \
     }                                        \
     break;
+    float e;
     switch (act) {
         case PSFM_ACT_RELU: PSFM_EACH(v < 0.0f ? 0.0f : v)     // NaN stays
         case PSFM_ACT_SIGMOID: PSFM_EACH(sigmoidf(v))
         case PSFM_ACT_ELU: PSFM_EACH(v > 0.0f ? v : expm1f(v))
-        case PSFM_ACT_SILU: PSFM_EACH(v / (1.0f + __expf(-v)))
-        case PSFM_ACT_GELU: PSFM_EACH(0.5f * v * (1.0f + erff(v * 0.70710678118654752f)))
+        case PSFM_ACT_SILU: PSFM_EACH(v * sigmoidf(v))
+        case PSFM_ACT_GELU: PSFM_EACH(v * normal_cdf<T>(v, e))
         default: break;
     }
 #undef PSFM_EACH
@@ -60,10 +79,13 @@ __device__ __forceinline__ float slope_sigmoid(float z) {
     const float s = sigmoidf(z);
     return s * (1.0f - s);
 }
+template <typename T>
 __device__ __forceinline__ float slope_gelu(float z) {
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    float e;
+    const float c = normal_cdf<T>(z, e);
+    return c + z * e * 0.39894228040143268f;
 }
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void times_slope(int act, const float (&z)[N], float (&d)[N]) {
 #define PSFM_EACH(F) \
     _Pragma("unroll") for (int k = 0; k < N; ++k) d[k] *= F; \
@@ -73,7 +95,7 @@ __device__ __forceinline__ void times_slope(int act, const float (&z)[N], float 
         case PSFM_ACT_SIGMOID: PSFM_EACH(slope_sigmoid(z[k]))
         case PSFM_ACT_ELU: PSFM_EACH((z[k] > 0.0f ? 1.0f : __expf(z[k])))
         case PSFM_ACT_SILU: PSFM_EACH(slope_silu(z[k]))
-        case PSFM_ACT_GELU: PSFM_EACH(slope_gelu(z[k]))
+        case PSFM_ACT_GELU: PSFM_EACH(slope_gelu<T>(z[k]))
         default: break;
     }
 #undef PSFM_EACH
@@ -150,24 +172,10 @@ __device__ __forceinline__ void load_run(const T* p, float (&v)[N], int n) {
     }
 }
 
-// v[k] = kept ? v[k] * scale : 0 for the columns j .. j + N - 1 (j % 4 = 0) of mask row mrow
-template <int N>
-__device__ __forceinline__ void drop_run(const DropArgs& d, const PhiloxKey& key, int64_t cols, int64_t mrow, int64_t j,
-                                         float scale, float (&v)[N]) {
-    const uint64_t block = mask_block(mrow, cols, j);
-#pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
-        uint32_t w[4];
-        philox4(key, block + q, w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[4 * q + k] = w[k] <= d.last ? 0.0f : v[4 * q + k] * scale;
-    }
-}
-
 // ---- the epilogue of columns j .. j + N - 1 (j % 4 = 0; those below J exist) of row i -----------------
 template <typename T, bool FULL, int N>
-__device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& key, int64_t J, int64_t i, int64_t j,
-                                         float (&v)[N]) {
+__device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& key, KeepBits<N>& keep, int64_t J, int64_t i,
+                                         int64_t j, float (&v)[N]) {
     const int n = J - j < N ? (int)(J - j) : N;
     const int64_t at = i * J + j;
     if (!FULL) {
@@ -195,8 +203,8 @@ __device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& ke
             store_run((Z*)e.z + at, v, n);
         }
     }
-    act_of(e.act, v);
-    if (e.drop.rng) drop_run(e.drop, key, J, mask_row(e.drop, i), j, e.drop.scale, v);
+    act_of<T>(e.act, v);
+    if (e.drop.rng) drop_run(e.drop, key, keep, J, mask_row(e.drop, i), j, e.drop.scale, v);
     if (e.res) {
         float r[N];
         load_run((const T*)e.res + i * e.ldr + j, r, n);
@@ -304,6 +312,7 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
     static constexpr int V = S::V, ZN = (int)sizeof(Z) * V / 16;
     u4v z[S::NC][ZN];
     float sum[V];
+    KeepBits<V> keep;
 
     __device__ __forceinline__ void load(const GemmArgs& A, int64_t b0, int64_t ext, int64_t r0, int64_t rend) {
         S::load((const T*)A.P, A.ldp, b0, ext, r0, rend);
@@ -350,12 +359,12 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
                         for (int k = 0; k < 16 / (int)sizeof(Z); ++k) zv[h * (16 / (int)sizeof(Z)) + k] = (float)zz[k];
                     }
                 }
-                times_slope(A.dz.act, zv, d);
+                times_slope<T>(A.dz.act, zv, d);
             }
             if (A.dz.drop.rng) {   // last: a dropped value is 0 whatever dy and z hold
                 int64_t row, col;
                 S::place(q, b0, r0, row, col);
-                drop_run(A.dz.drop, key, A.ldp, mask_row(A.dz.drop, row), col, 1.0f, d);
+                drop_run(A.dz.drop, key, keep, A.ldp, mask_row(A.dz.drop, row), col, 1.0f, d);
             }
             TV o;
 #pragma unroll
@@ -617,6 +626,7 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     float* tile = reinterpret_cast<float*>(&stage0[0]);
     PhiloxKey key{};
     if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
+    KeepBits<V> keep;
     const int col = threadIdx.x % CPR * V;
 #pragma unroll
     for (int band = 0; band < BANDS; ++band) {
@@ -643,7 +653,7 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[4 * q + k] = x[k];
                 }
-                epilogue<T, FULL>(A.e, key, A.J, ib + i, j0 + col, v);
+                epilogue<T, FULL>(A.e, key, keep, A.J, ib + i, j0 + col, v);
             }
         }
     }
@@ -658,19 +668,20 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_forward(const GemmArgs A) {
 template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DZ>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_pair(const PairArgs A) {
     __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128];
-    if (blockIdx.x < A.ndx)
-        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ>(A.dx, blockIdx.x, A.ndx, stage0, stage1);
+    if (blockIdx.x < A.ndw)
+        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ>(A.dw, blockIdx.x, A.ndw, stage0, stage1);
     else
-        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ>(A.dw, blockIdx.x - A.ndx, A.ndw, stage0, stage1);
+        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ>(A.dx, blockIdx.x - A.ndw, A.ndx, stage0, stage1);
 }
 
-// y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction, 64 bytes of each row a step; each reads
-// 16 rows of W straight into the matrix instructions' operands, U steps in flight, and x's few rows from the caches.
+// y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction, 128 bytes of each row (two steps) a
+// turn; each reads 16 rows of W straight into the matrix instructions' operands, U steps in flight, and x's few rows
+// from the caches.
 constexpr int SKINNY_WAVES = 8;
 
 template <typename T, int MT, bool VEC>
 __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A) {
-    constexpr int V = CHUNK<T>, STEP = 4 * V, U = 8 / MT;
+    constexpr int V = CHUNK<T>, STEP = 4 * V, U = 16 / MT;
     __shared__ f4 part[SKINNY_WAVES][MT][64];
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4, n = l & 15;
     const int64_t j0 = (int64_t)blockIdx.x * 16, j = j0 + n;
@@ -678,11 +689,11 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
     f4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = f4{0, 0, 0, 0};
-    for (int64_t k0 = (int64_t)wave * STEP; k0 < A.K; k0 += SKINNY_WAVES * U * STEP) {
+    for (int64_t k0 = (int64_t)wave * 2 * STEP; k0 < A.K; k0 += SKINNY_WAVES * U * STEP) {
         u4v fw[U], fx[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t k = k0 + u * SKINNY_WAVES * STEP + g * V, left = A.K - k;
+            const int64_t k = k0 + (u / 2 * 2 * SKINNY_WAVES + u % 2) * STEP + g * V, left = A.K - k;
             const int have = left >= V ? V : left > 0 ? (int)left : 0;
             fw[u] = load_n<T, VEC>(w + (have ? k : 0), j < A.N ? have : 0);
 #pragma unroll
@@ -710,7 +721,8 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
     for (int s = 0; s < SKINNY_WAVES; ++s)
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] += part[s][wave][l][k];
-    epilogue<T, true>(A.e, key, A.N, i, jj, v);
+    KeepBits<4> keep;
+    epilogue<T, true>(A.e, key, keep, A.N, i, jj, v);
 }
 
 // Split products: 256 / SL groups of four columns a workgroup, SL threads a group, each summing every SL-th split;
@@ -746,7 +758,8 @@ __device__ __forceinline__ void join(const GemmArgs& A, uint32_t block, f4* sums
     if (!in) return;
     PhiloxKey key{};
     if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
-    epilogue<T, FULL>(A.e, key, A.J, i, j, v);
+    KeepBits<4> keep;
+    epilogue<T, FULL>(A.e, key, keep, A.J, i, j, v);
 }
 
 constexpr int JOIN_FEW = 8, JOIN_LANES = 16;   // up to JOIN_FEW splits one thread a group sums them all
@@ -806,6 +819,7 @@ __global__ __launch_bounds__(DZ_THREADS) void k_dz(const DzPassArgs A) {
     const DropArgs& drop = A.dz.drop;
     PhiloxKey key{};
     if (drop.rng) key = philox_key(drop.rng);
+    KeepBits<V> keep;
     float sum[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) sum[k] = 0;
@@ -819,10 +833,10 @@ __global__ __launch_bounds__(DZ_THREADS) void k_dz(const DzPassArgs A) {
                     load_run((const T*)A.dz.z + m * A.N + j, z, n);
                 else
                     load_run((const typename KeptZ<T>::type*)A.dz.z + m * A.N + j, z, n);
-                times_slope(A.dz.act, z, d);
+                times_slope<T>(A.dz.act, z, d);
             }
             // last: a dropped value is 0 whatever dy and z hold
-            if (drop.rng) drop_run(drop, key, A.N, mask_row(drop, m), j, 1.0f, d);
+            if (drop.rng) drop_run(drop, key, keep, A.N, mask_row(drop, m), j, 1.0f, d);
             if (A.out) store_run((T*)A.out + m * A.N + j, d, n);
 #pragma unroll
             for (int k = 0; k < V; ++k) sum[k] += d[k];

@@ -55,6 +55,57 @@ __device__ __forceinline__ uint64_t mask_block(int64_t mrow, int64_t cols, int64
     return (uint64_t)mrow * (uint64_t)((cols + 3) >> 2) + (uint64_t)(j >> 2);
 }
 
+// v[k] = kept ? v[k] * scale : 0 for the N columns of the mask block `block` and the next ones.
+template <int N>
+__device__ __forceinline__ void drop_block(const DropArgs& d, const PhiloxKey& key, uint64_t block, float scale,
+                                           float (&v)[N]) {
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        uint32_t w[4];
+        philox4(key, block + q, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * q + k] = w[k] <= d.last ? 0.0f : v[4 * q + k] * scale;
+    }
+}
+
+// The keep bits of N columns, kept from call to call: a mask by channel is the same from row to row, and made anew only
+// where the block is another.  A mask by element always is another, and goes by drop_block: the bits'
+// packing and the branch cost a tenth of a pass there.
+template <int N>
+struct KeepBits {
+    uint64_t block = ~0ull;
+    uint32_t bits = 0;
+
+    __device__ __forceinline__ uint32_t at(const DropArgs& d, const PhiloxKey& key, uint64_t b) {
+        if (b != block) {
+            block = b;
+            bits = 0;
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) {
+                uint32_t w[4];
+                philox4(key, b + q, w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bits |= (w[k] <= d.last ? 0u : 1u) << (4 * q + k);
+            }
+        }
+        return bits;
+    }
+};
+
+// The same of the columns j .. j + N - 1 (j % 4 = 0) of mask row mrow
+template <int N>
+__device__ __forceinline__ void drop_run(const DropArgs& d, const PhiloxKey& key, KeepBits<N>& keep, int64_t cols,
+                                         int64_t mrow, int64_t j, float scale, float (&v)[N]) {
+    const uint64_t block = mask_block(mrow, cols, j);
+    if (d.mask_rows == 1) {
+        drop_block(d, key, block, scale, v);
+    } else {
+        const uint32_t bits = keep.at(d, key, block);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = bits >> k & 1 ? v[k] * scale : 0.0f;
+    }
+}
+
 // The host side of a mask: the words 0 .. last drop, so that round(p 2^32) of 2^32 do.  False where p drops
 // nothing at that resolution.  p = 1 drops everything; its scale is never used and stays finite.
 inline bool drop_threshold(double p, uint32_t* last, float* scale) {

@@ -1,6 +1,7 @@
 """PackNet01 (packnet_sfm/networks/depth/PackNet01.py:8-185): 3D packing encoder / unpacking
 decoder with inverse-depth heads at 4 scales.  Versions '1A' (skip concatenation) and '1B'
-(skip addition).  Module names follow the reference (checkpoint compatible)."""
+(skip addition).  Module names follow the reference (checkpoint compatible).  dropout_seed: the
+residual blocks' channel dropout from the counter-based generator (layers01.ResidualConv)."""
 import torch
 import torch.nn as nn
 
@@ -10,7 +11,7 @@ from ..layers.packnet.layers01 import (Conv2D, InvDepth, PackLayerConv3d, Residu
 
 
 class PackNet01(nn.Module):
-    def __init__(self, dropout=None, version=None, **kwargs):
+    def __init__(self, dropout=None, version=None, dropout_seed=None, **kwargs):
         super().__init__()
         self.version = version[1:]
         ni, no = 64, 1
@@ -34,10 +35,10 @@ class PackNet01(nn.Module):
         self.pack4 = PackLayerConv3d(n4, pack_k[3])
         self.pack5 = PackLayerConv3d(n5, pack_k[4])
         self.conv1 = Conv2D(ni, n1, 7, 1)
-        self.conv2 = ResidualBlock(n1, n2, num_blocks[0], 1, dropout=dropout)
-        self.conv3 = ResidualBlock(n2, n3, num_blocks[1], 1, dropout=dropout)
-        self.conv4 = ResidualBlock(n3, n4, num_blocks[2], 1, dropout=dropout)
-        self.conv5 = ResidualBlock(n4, n5, num_blocks[3], 1, dropout=dropout)
+        self.conv2 = ResidualBlock(n1, n2, num_blocks[0], 1, dropout, dropout_seed, 2 << 40)
+        self.conv3 = ResidualBlock(n2, n3, num_blocks[1], 1, dropout, dropout_seed, 3 << 40)
+        self.conv4 = ResidualBlock(n3, n4, num_blocks[2], 1, dropout, dropout_seed, 4 << 40)
+        self.conv5 = ResidualBlock(n4, n5, num_blocks[3], 1, dropout, dropout_seed, 5 << 40)
         self.unpack5 = UnpackLayerConv3d(n5, outs[5], unpack_k[0])
         self.unpack4 = UnpackLayerConv3d(n5, outs[4], unpack_k[1])
         self.unpack3 = UnpackLayerConv3d(n4, outs[3], unpack_k[2])

@@ -10,7 +10,8 @@ fusion parameters `weight` / `bias` [5] are kept (unused on the RGB path, as in 
 they get no gradient) so parameter names and counts match; a reference checkpoint loads with
 `load_state_dict(strict=False)` minus its `mconvs.*` entries.
 
-Module names follow the reference (`encoder.*`, `decoder.*`).  The pack / unpack 3-D
+dropout_seed: the residual blocks' channel dropout from the counter-based generator
+(layers01.ResidualConv).  Module names follow the reference (`encoder.*`, `decoder.*`).  The pack / unpack 3-D
 convolutions run on the fused HIP kernels (layers01.PackLayerConv3d / UnpackLayerConv3d, d = 4).
 """
 import torch
@@ -25,7 +26,7 @@ class Encoder(nn.Module):
     """PackNetSAN01.py:11-50."""
 
     def __init__(self, version, in_channels, ni, n1, n2, n3, n4, n5, pack_kernel, num_blocks, num_3d_feat,
-                 dropout):
+                 dropout, dropout_seed=None):
         super().__init__()
         self.version = version
         self.pre_calc = Conv2D(in_channels, ni, 5, 1)
@@ -35,10 +36,10 @@ class Encoder(nn.Module):
         self.pack4 = PackLayerConv3d(n4, pack_kernel[3], d=num_3d_feat)
         self.pack5 = PackLayerConv3d(n5, pack_kernel[4], d=num_3d_feat)
         self.conv1 = Conv2D(ni, n1, 7, 1)
-        self.conv2 = ResidualBlock(n1, n2, num_blocks[0], 1, dropout=dropout)
-        self.conv3 = ResidualBlock(n2, n3, num_blocks[1], 1, dropout=dropout)
-        self.conv4 = ResidualBlock(n3, n4, num_blocks[2], 1, dropout=dropout)
-        self.conv5 = ResidualBlock(n4, n5, num_blocks[3], 1, dropout=dropout)
+        self.conv2 = ResidualBlock(n1, n2, num_blocks[0], 1, dropout, dropout_seed, 2 << 40)
+        self.conv3 = ResidualBlock(n2, n3, num_blocks[1], 1, dropout, dropout_seed, 3 << 40)
+        self.conv4 = ResidualBlock(n3, n4, num_blocks[2], 1, dropout, dropout_seed, 4 << 40)
+        self.conv5 = ResidualBlock(n4, n5, num_blocks[3], 1, dropout, dropout_seed, 5 << 40)
 
     def forward(self, rgb):
         x = self.pre_calc(rgb)
@@ -105,7 +106,7 @@ class Decoder(nn.Module):
 class PackNetSAN01(nn.Module):
     """PackNetSAN01.py:143-235 (RGB path)."""
 
-    def __init__(self, dropout=None, version=None, **kwargs):
+    def __init__(self, dropout=None, version=None, dropout_seed=None, **kwargs):
         super().__init__()
         self.version = version[1:]
         in_channels, out_channels = 3, 1
@@ -114,7 +115,7 @@ class PackNetSAN01(nn.Module):
         pack_kernel, unpack_kernel, iconv_kernel = [5, 3, 3, 3, 3], [3] * 5, [3] * 5
         num_3d_feat = 4
         self.encoder = Encoder(self.version, in_channels, ni, n1, n2, n3, n4, n5, pack_kernel, num_blocks,
-                               num_3d_feat, dropout)
+                               num_3d_feat, dropout, dropout_seed)
         self.decoder = Decoder(self.version, out_channels, ni, n1, n2, n3, n4, n5, unpack_kernel, iconv_kernel,
                                num_3d_feat)
         self.mconvs = None   # MinkowskiEncoder (SAN LiDAR branch): out of scope, see module docstring

@@ -24,6 +24,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from ... import _hip
+from ...utils.horovod import rank
 
 
 class Drop(NamedTuple):
@@ -191,31 +192,39 @@ def dropout2d(x, drop, residual=None):
 
 class CounterDropout(nn.Module):
     """Dropout whose masks are (seed, offset), the offset counted on the device: in training every forward draws
-    the next one, also in a captured graph's replays.  Data-parallel ranks and the layers of one network take
-    different seeds or first offsets.  The state is no part of the state_dict: checkpoints of networks with
-    nn.Dropout load as they are."""
+    the next one, also in a captured graph's replays.  The ranks of a data-parallel job, which hold the same
+    buffers, take seed + rank; the layers of one network take different first offsets.  The state is no part
+    of the state_dict: checkpoints of networks with nn.Dropout load as they are."""
 
     def __init__(self, p, seed, offset=0, channels=False):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability {p} is not in 0 .. 1")
         self.p, self.channels = float(p), channels
-        wrap = [(int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63 for v in (seed, offset)]
-        self.register_buffer("state", torch.tensor(wrap, dtype=torch.int64), persistent=False)
+        self.register_buffer("state", torch.tensor([_int64(seed), _int64(offset)]), persistent=False)
+
+    def extra_repr(self):
+        return f"p={self.p}, channels={self.channels}"
 
     def draw(self):
         """The Drop of this forward (None where nothing is dropped)."""
         if not self.training or self.p == 0.0:
             return None
-        if not self.state.is_cuda:
-            used = self.state.clone()
-            self.state[1] += 1
-            return Drop(self.p, used, self.channels)
-        used = torch.empty_like(self.state)
-        with on_device(self.state.device):
-            _hip.check(_hip.lib().psfm_rng_next(_hip.ptr(self.state), _hip.ptr(used), _hip.stream(self.state.device)),
+        state = self.state
+        if not state.is_cuda:
+            seed, offset = state.tolist()
+            state[1] = _int64(offset + 1)
+            return Drop(self.p, torch.tensor([_int64(seed + rank()), offset]), self.channels)
+        used = torch.empty_like(state)
+        with on_device(state.device):
+            _hip.check(_hip.lib().psfm_rng_next(state.data_ptr(), rank(), used.data_ptr(), _hip.stream(state.device)),
                        "psfm_rng_next")
         return Drop(self.p, used, self.channels)
 
     def forward(self, x, residual=None):
         return (dropout2d if x.dim() == 4 else dropout)(x, self.draw(), residual)
+
+
+def _int64(v):
+    """v of 64 bits as the signed number of the same bits."""
+    return (int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63

@@ -10,7 +10,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..dropout import CounterDropout
 from ..fused import ACT_ELU, gn_act
+from ..linear import conv1x1_act
 from . import packconv
 from .pack3d import conv3d_unpack, pack_conv3d
 
@@ -37,14 +39,21 @@ class Conv2D(nn.Module):
 
 
 class ResidualConv(nn.Module):
-    """Two Conv2D + 1x1 shortcut, GroupNorm + ELU after the sum."""
+    """Two Conv2D + 1x1 shortcut, GroupNorm + ELU after the sum.
 
-    def __init__(self, in_channels, out_channels, stride, dropout=None):
+    dropout drops whole channels of the shortcut.  With dropout_seed the masks come from the counter-based
+    generator (dropout.CounterDropout: repeatable from the seed, nothing stored for the backward pass)
+    and the shortcut is one pass: conv2's branch + drop(1x1 convolution + bias) in its epilogue."""
+
+    def __init__(self, in_channels, out_channels, stride, dropout=None, dropout_seed=None, dropout_offset=0):
         super().__init__()
         self.conv1 = Conv2D(in_channels, out_channels, 3, stride)
         self.conv2 = Conv2D(out_channels, out_channels, 3, 1)
         shortcut = nn.Conv2d(in_channels, out_channels, kernel_size=1, stride=stride)
-        self.conv3 = nn.Sequential(shortcut, nn.Dropout2d(dropout)) if dropout else shortcut
+        if dropout and dropout_seed is not None:
+            self.conv3 = nn.Sequential(shortcut, CounterDropout(dropout, dropout_seed, dropout_offset, channels=True))
+        else:
+            self.conv3 = nn.Sequential(shortcut, nn.Dropout2d(dropout)) if dropout else shortcut
         self.normalize = nn.GroupNorm(16, out_channels)
         self.activ = nn.ELU(inplace=True)
 
@@ -54,13 +63,18 @@ class ResidualConv(nn.Module):
         if isinstance(self.conv3, nn.Conv2d):
             c = self.conv3
             return gn_act(F.conv2d(x, c.weight, None, c.stride), c.bias, self.normalize, act=ACT_ELU, residual=r)
+        if isinstance(self.conv3[1], CounterDropout):
+            c, drop = self.conv3
+            x = x if c.stride == (1, 1) else x[..., ::c.stride[0], ::c.stride[1]]
+            h = conv1x1_act(x, c.weight, c.bias, residual=r, drop=drop.draw())
+            return gn_act(h, None, self.normalize, act=ACT_ELU)
         return gn_act(self.conv3(x), None, self.normalize, act=ACT_ELU, residual=r)
 
 
-def ResidualBlock(in_channels, out_channels, num_blocks, stride, dropout=None):
-    blocks = [ResidualConv(in_channels, out_channels, stride, dropout=dropout)]
-    blocks += [ResidualConv(out_channels, out_channels, 1, dropout=dropout) for _ in range(1, num_blocks)]
-    return nn.Sequential(*blocks)
+def ResidualBlock(in_channels, out_channels, num_blocks, stride, dropout=None, dropout_seed=None, dropout_offset=0):
+    """dropout_seed, dropout_offset: block b counts its masks from dropout_offset + b * 2^32."""
+    return nn.Sequential(*[ResidualConv(in_channels if b == 0 else out_channels, out_channels, stride if b == 0 else 1,
+                                        dropout, dropout_seed, dropout_offset + (b << 32)) for b in range(num_blocks)])
 
 
 class InvDepth(nn.Module):

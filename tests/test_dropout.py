@@ -289,4 +289,4 @@ def test_refusals():
         assert L.psfm_dropout(*args, None) == code, args
         assert L.psfm_dropout_last_error()
     assert L.psfm_dropout(a, 4, None, 0, 0, 0, 4, 1, 0.5, a, a, None) == 0      # nothing to do
-    assert L.psfm_rng_next(None, a, None) == -1
+    assert L.psfm_rng_next(None, 0, a, None) == -1 and L.psfm_rng_next(a, 0, None, None) == -1

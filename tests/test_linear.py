@@ -488,9 +488,12 @@ def test_refusals():
     assert L.psfm_linear_fwd(ctypes.byref(d), a, a, None, a, a, None, None, None) == -3
     d = _hip.Linear(**{**good, "act": LI.ACT_SILU})
     assert L.psfm_linear_bwd(ctypes.byref(d), a, a, a, None, a, None, None, a, None) == -9     # no z
-    assert L.psfm_linear_bwd(ctypes.byref(d), a, a, a, a, a, None, None, None, None) == -10    # no workspace
-    d = _hip.Linear(**{**good, "M": 4, "K": 65536, "ldx": 65536})
-    assert L.psfm_linear_fwd_ws_bytes(ctypes.byref(d)) >= 0
+    d = _hip.Linear(**{**good, "act": LI.ACT_SILU, "M": 100000})   # a long reduction is split: no workspace
+    assert L.psfm_linear_bwd_ws_bytes(ctypes.byref(d), 0, 1, 0) > 0
+    assert L.psfm_linear_bwd(ctypes.byref(d), a, a, a, a, None, a, None, None, None) == -10
+    d = _hip.Linear(**{**good, "M": 64, "K": 65536, "ldx": 65536})
+    assert L.psfm_linear_fwd_ws_bytes(ctypes.byref(d)) > 0
+    assert L.psfm_linear_fwd(ctypes.byref(d), a, a, None, None, a, None, None, None) == -10
     assert L.psfm_linear_fwd(None, a, a, None, None, a, None, a, None) == -1
     d = _hip.Linear(**{**good, "M": 0})
     assert L.psfm_linear_fwd(ctypes.byref(d), None, a, None, None, None, None, None, None) == 0
