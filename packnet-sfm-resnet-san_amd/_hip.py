@@ -224,6 +224,31 @@ def lib():
     return L
 
 
+EXT_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_psfm_autograd.so")
+_ext = None
+
+
+def ext():
+    """The autograd nodes in C++ (csrc/psfm_autograd.cpp), loaded once beside the library whose entry points they call."""
+    global _ext
+    if _ext is None:
+        import importlib.machinery
+        import importlib.util
+        L, G = lib(), _graft_entry()
+        if G.library_hash(EXT_PATH, G.EXT_TAG) != G.source_hash():
+            raise RuntimeError(f"{EXT_PATH} is not built from the tree's sources: run __graft_entry__.build()")
+        loader = importlib.machinery.ExtensionFileLoader("_psfm_autograd", EXT_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_psfm_autograd", loader))
+        loader.exec_module(mod)
+        names = ("psfm_linear_fwd_ws_bytes", "psfm_linear_fwd", "psfm_linear_bwd_ws_bytes", "psfm_linear_bwd",
+                 "psfm_linear_last_error", "psfm_dropout", "psfm_dropout_last_error")
+        with _CAPTURE_LOCK:
+            if _ext is None:
+                mod.init({n: ctypes.cast(getattr(L, n), c_void_p).value for n in names}, _foreign_capture, _ACTIVE_CAPTURES)
+                _ext = mod
+    return _ext
+
+
 EXPORTED = ("psfm_workspace_floats", "psfm_photometric_clip_stats", "psfm_photometric_fwd",
             "psfm_smoothness_fwd", "psfm_finalize", "psfm_photometric_bwd", "psfm_smoothness_bwd",
             "psfm_pose_grad_reduce", "psfm_photometric_prepass", "psfm_photometric_fwd_grad", "psfm_photometric_grad_finish",
@@ -338,6 +363,8 @@ def _install_capture_hooks():
         with _CAPTURE_LOCK:
             _ACTIVE_CAPTURES += 1
             _CAPTURE_STREAMS.append(torch.cuda.current_stream())
+            if _ext is not None:
+                _ext.set_captures(_ACTIVE_CAPTURES)
         return r
 
     def capture_end(self, *a, **k):
@@ -346,6 +373,8 @@ def _install_capture_hooks():
             _ACTIVE_CAPTURES = max(0, _ACTIVE_CAPTURES - 1)
             if _CAPTURE_STREAMS:
                 _CAPTURE_STREAMS.pop()
+            if _ext is not None:
+                _ext.set_captures(_ACTIVE_CAPTURES)
         return end(self, *a, **k)
 
     G.capture_begin, G.capture_end, G._psfm_counted = capture_begin, capture_end, True
@@ -358,10 +387,6 @@ def _install_capture_hooks():
 # then segfaults in capture_end — by the time the op's own backward runs, the autograd engine has
 # already recorded that wait, so the refusal has to come before the capture exists.
 _EAGER_CTX = weakref.WeakSet()
-# Contexts whose backward has run, whose graph still lives (its output is held) and whose forward ran on the
-# default stream: the graph keeps its leaves' gradient accumulators, which are bound to that stream, and a
-# captured backward of the same leaves would accumulate there; the default stream cannot join a capture.
-_EAGER_DONE = weakref.WeakSet()
 
 
 def note_forward(ctx):
@@ -385,11 +410,17 @@ def _refuse_stray_backward(cap_stream):
             "backpropagated; a backward captured for them would run on their forward's stream, outside the "
             "capture (HIP segfaults in capture_end).  Run the backward (or free the graph) first, or run the "
             "forward inside the same capture, as DDPTrainer.capture does")
-    with _CAPTURE_LOCK:
-        held = sorted({type(c).__name__ for c in list(_EAGER_DONE)})
+    if _ext is None:
+        return
+    pending, held = _ext.alive(cap_stream.cuda_stream)
+    if pending:
+        raise RuntimeError(
+            f"psfm: refusing to begin a HIP-graph capture on stream {cap_stream.cuda_stream:#x}: {pending} forward(s) of "
+            "linear_act / dropout ran outside any capture on another stream and can still be backpropagated.  Run the "
+            "backward (or free the graph) first, or run the forward inside the same capture")
     if held:
         raise RuntimeError(
-            f"psfm: refusing to begin a HIP-graph capture while outputs of {', '.join(held)} from an eager step on the "
+            "psfm: refusing to begin a HIP-graph capture while outputs of linear_act / dropout from an eager step on the "
             "default stream are held: their graphs keep the leaves' gradient accumulators on that stream, which a "
             "captured backward cannot use.  Free those outputs first (or run the eager steps on a side stream)")
 
@@ -397,36 +428,38 @@ def _refuse_stray_backward(cap_stream):
 _install_capture_hooks()
 
 
-def capture_guard(ctx=None, leaves=False):
+def capture_guard(ctx=None):
     """Raise before anything is allocated or launched when this thread is not capturing while a
     HIP-graph capture is in progress — called first thing in every HIP backward: PyTorch-ROCm runs a
     node's backward on its forward's stream, so a backward captured for a forward that ran outside
     the capture would otherwise allocate and launch on a stream the capture does not own, and HIP
     segfaults in capture_end.  `ctx` (the op's autograd context) leaves
     the set of pending eager forwards (note_forward) here.  The capture_begin hook refuses such a
-    capture before it starts; this check is the last line for anything it cannot see.  `leaves`: the
-    context goes on being watched for the leaves that its graph holds (_EAGER_DONE)."""
+    capture before it starts; this check is the last line for anything it cannot see."""
     if ctx is not None:
         with _CAPTURE_LOCK:
             _EAGER_CTX.discard(ctx)
-            if leaves and getattr(ctx, "_psfm_stream", None) == 0:
-                _EAGER_DONE.add(ctx)
     if _ACTIVE_CAPTURES and not torch.cuda.is_current_stream_capturing():
-        # Refuse — but first join this stream into the capture and straight back (an empty fork), so
-        # the capture is still well formed when the error unwinds through torch.cuda.graph: the
-        # autograd engine syncs the backward's stream with the caller's (capturing) stream on the way
-        # out, and a wait on a stream outside the capture makes HIP's capture_end segfault.
-        cur = torch.cuda.current_stream()
-        cap = _CAPTURE_STREAMS[-1] if _CAPTURE_STREAMS else None
-        if cap is not None and cap.cuda_stream != cur.cuda_stream:
-            cur.wait_stream(cap)
-            cap.wait_stream(cur)
-        raise RuntimeError(
-            "psfm: a HIP op would run on a stream outside the HIP-graph capture in progress (stream "
-            f"{torch.cuda.current_stream().cuda_stream:#x} is not capturing).  This happens when an op's "
-            "backward is captured but its forward ran on another stream (autograd runs the backward on "
-            "the forward's stream): run the forward inside the same capture (or on the capture stream), "
-            "as DDPTrainer.capture does")
+        raise RuntimeError(_foreign_capture())
+
+
+def _foreign_capture():
+    """Make the capture in progress well formed again; the message of its refusal."""
+    # first join this stream into the capture and straight back (an empty fork), so
+    # the capture is still well formed when the error unwinds through torch.cuda.graph: the
+    # autograd engine syncs the backward's stream with the caller's (capturing) stream on the way
+    # out, and a wait on a stream outside the capture makes HIP's capture_end segfault.
+    cur = torch.cuda.current_stream()
+    cap = _CAPTURE_STREAMS[-1] if _CAPTURE_STREAMS else None
+    if cap is not None and cap.cuda_stream != cur.cuda_stream:
+        cur.wait_stream(cap)
+        cap.wait_stream(cur)
+    return (
+        "psfm: a HIP op would run on a stream outside the HIP-graph capture in progress (stream "
+        f"{torch.cuda.current_stream().cuda_stream:#x} is not capturing).  This happens when an op's "
+        "backward is captured but its forward ran on another stream (autograd runs the backward on "
+        "the forward's stream): run the forward inside the same capture (or on the capture stream), "
+        "as DDPTrainer.capture does")
 
 
 def stream(device):

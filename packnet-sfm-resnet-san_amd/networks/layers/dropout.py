@@ -14,14 +14,13 @@ again and neither stores it, and a run can be repeated from its seed whatever el
 
 linear.linear_act takes the same Drop into its epilogue: the mask is the one that `dropout` would
 give its output.  fp32, fp16 and bf16 tensors on a ROCm device run the HIP kernel; anything else
-(CPU tensors, fp64) runs the same arithmetic as plain torch ops.
+(CPU tensors, fp64) runs the same arithmetic as plain torch ops.  The autograd nodes are in C++ (csrc/psfm_autograd.cpp).
 """
 from contextlib import nullcontext
 from typing import NamedTuple
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from ... import _hip
 from ...utils.horovod import rank
@@ -54,38 +53,6 @@ def mask_rows(shape, channels):
     for s in shape[1:-1]:
         n *= s
     return max(n, 1)
-
-
-def row_stride(t):
-    """The stride between consecutive rows of t as a [rows, last dimension] matrix, or None where it has no
-    such form (columns apart, rows at uneven distances)."""
-    cols = t.shape[-1]
-    if t.is_contiguous():
-        return cols
-    if t.stride(-1) != 1 and cols != 1:
-        return None
-    ld = None
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size == 1:
-            continue
-        if ld is None:
-            ld, reach = stride, stride * size
-        elif stride == reach:
-            reach = stride * size
-        else:
-            return None
-    if ld is None:
-        return cols
-    return ld if ld >= cols else None
-
-
-def as_rows(t):
-    """(t, its row stride), copied only where it has none."""
-    ld = row_stride(t)
-    if ld is None:
-        t = t.contiguous()
-        ld = t.shape[-1]
-    return t, ld
 
 
 _HERE = nullcontext()
@@ -123,37 +90,6 @@ def plain_drop(t, drop):
     return torch.where(keep.unsqueeze(1), t.reshape(-1, share, shape[-1]) * scale, 0.0).view(shape)
 
 
-def _launch(x, residual, p, rng, share):
-    x, ldx = as_rows(x)
-    res, ldr = (None, 0) if residual is None else as_rows(residual)
-    cols = x.shape[-1]
-    device, dtype, n = x.device, x.dtype, x.numel()
-    y = torch.empty(x.shape, device=device, dtype=dtype)
-    if n:
-        with on_device(device):
-            _hip.check(_hip.lib().psfm_dropout(x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr,
-                                               _hip.DTYPES[dtype], n // cols, cols, share, p, rng.data_ptr(),
-                                               y.data_ptr(), _hip.stream(device)), "psfm_dropout")
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, rng, share):
-        _hip.note_forward(ctx)
-        ctx.save_for_backward(rng)
-        ctx.p, ctx.share = p, share
-        return _launch(x, residual, p, rng, share)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        _hip.capture_guard(ctx, leaves=True)
-        (rng,) = ctx.saved_tensors
-        dx = _launch(dy, None, ctx.p, rng, ctx.share) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
-
-
 def check_like(t, name, shape, x):
     if t.shape != shape or t.dtype != x.dtype or t.device != x.device:
         raise RuntimeError(f"{name} must be {tuple(shape)} {x.dtype} on {x.device}; got {tuple(t.shape)} {t.dtype} on "
@@ -175,10 +111,7 @@ def dropout(x, drop, residual=None):
         wide = torch.promote_types(x.dtype, torch.float32)
         y = plain_drop(x.to(wide), drop)
         return (y if residual is None else y + residual.to(wide)).to(x.dtype)
-    share = mask_rows(x.shape, drop.channels)
-    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
-        return _Dropout.apply(x, residual, drop.p, drop.rng, share)
-    return _launch(x, residual, drop.p, drop.rng, share)
+    return _hip.ext().dropout(x, residual, drop.p, drop.rng, drop.channels)
 
 
 def dropout2d(x, drop, residual=None):

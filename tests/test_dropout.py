@@ -10,7 +10,7 @@ import torch
 
 import packnet_sfm_amd  # noqa: F401
 from packnet_sfm_amd import _hip
-from packnet_sfm_amd.networks.layers.dropout import CounterDropout, Drop, dropout, dropout2d, keep_mask, row_stride
+from packnet_sfm_amd.networks.layers.dropout import CounterDropout, Drop, dropout, dropout2d, keep_mask
 
 gpu = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -252,14 +252,6 @@ def test_plain_path_on_the_cpu():
     a, b = m(torch.ones(2, 3, 5)), m(torch.ones(2, 3, 5))
     assert np.array_equal((a[:, 0] != 0).numpy(), oracle_mask(2, 5, 0.4, 8, 9))
     assert np.array_equal((b[:, 0] != 0).numpy(), oracle_mask(2, 5, 0.4, 8, 10))
-
-
-def test_row_strides():
-    t = torch.zeros(4, 6, 10)
-    assert row_stride(t) == 10 and row_stride(t[..., :7]) == 10 and row_stride(t[:, 0]) == 60
-    assert row_stride(t[:, :5]) is None and row_stride(t[..., ::2]) is None and row_stride(t.transpose(0, 1)) is None
-    assert row_stride(t[:1, :5]) == 10 and row_stride(t[0, 0]) == 10 and row_stride(t[:, :1, 3:]) == 60
-    assert row_stride(torch.zeros(1, 10).expand(5, 10)) is None
 
 
 def test_refusals():
