@@ -59,9 +59,10 @@ struct Plan {
 };
 
 // Tiles: the largest that still fills the 256 CUs and computes at most an eighth more than the smallest
-// would (a 64-column layer in 256-column tiles: 86 us, 42 in 128), else the smallest.  The reduction is split while
-// the tiles alone leave CUs idle and a split keeps at least four LDS stages.
-Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1, int64_t fill = 512) {
+// would (a 64-column layer in 256-column tiles: 86 us, 42 in 128), else the smallest.  A long reduction is split while
+// that leaves every CU fewer than `fill` / 256 workgroups and a split keeps eight LDS stages, four where the tiles
+// alone leave CUs idle.
+Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1, int64_t fill = 768) {
     Plan p{0, 0, 0, 0, 1};
     const Tile& t0 = LINEAR_TILES[0];
     const double least = (double)(up(I, t0.bi) * t0.bi) * (double)(up(J, t0.bj) * t0.bj);
@@ -72,7 +73,8 @@ Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILE
     }
     const int64_t stage = 128 / size_of(dtype), stages = up(R, stage), tiles = p.ti * p.tj;
     int64_t splits = 1;
-    if (tiles > 0 && tiles < 256) splits = std::max<int64_t>(1, std::min(up(fill, tiles), stages / 4));
+    if (tiles > 0 && p.variant == 0)
+        splits = std::max<int64_t>(1, std::min(tiles < 256 ? up(fill, tiles) : fill / tiles, stages / (tiles < 256 ? 4 : 8)));
     const int64_t per = std::max<int64_t>(1, up(stages, splits));
     p.rsplit = per * stage;
     p.splits = (int)std::max<int64_t>(1, up(stages, per));
@@ -125,7 +127,7 @@ BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db)
     b.stage = any && (b.dx || b.dw) && cheap && (make || (want_db && b.dw));
     const int largest = b.stage ? 0 : LINEAR_NTILES - 1;
     if (b.dx) b.pdx = plan(d->dtype, d->M, d->K, d->N, largest);
-    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M, largest, b.dx ? 256 : 512);
+    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M, largest, b.dx ? 256 : 768);
     b.pass = any && !b.stage && ((make && (b.dx || b.dw)) || want_db);
     if (b.stage && want_db && !b.dw) b.pass = true;      // the column sums alone
     b.dz = b.pass && !b.stage && make && (b.dx || b.dw);

@@ -244,7 +244,28 @@ struct Stager {
         const int64_t left = row < (TURNED ? rend : ext) ? (TURNED ? ext : rend) - col : 0;
         return left >= V ? V : left > 0 ? (int)left : 0;
     }
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t b0, int64_t ext, int64_t r0, int64_t rend) {
+    // Whether every chunk of a stage may be read whole: the reduction does not end inside it, and where a chunk reaches
+    // over its row's end (turned: the tile's last columns, by V - 1 values at most; what it takes from there is
+    // never stored) there is as much of the operand behind the stage's last row.
+    static __device__ __forceinline__ bool whole(int64_t ld, int64_t b0, int64_t ext, int64_t r0, int64_t rend, int64_t all) {
+        constexpr int BR = 128 / (int)sizeof(T);
+        return r0 + BR <= rend && (!TURNED || b0 + B <= ext || (all - r0 - BR) * ld >= V - 1);
+    }
+    // all: the reduction's end in the operand, behind this split's too
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t b0, int64_t ext, int64_t r0, int64_t rend,
+                                         int64_t all) {
+        // uniform: no bounds a chunk (aligned chunks are whole or none, and reading the none ones costs more)
+        if (!VEC && whole(ld, b0, ext, r0, rend, all)) {
+#pragma unroll
+            for (int q = 0; q < NC; ++q) {
+                int64_t row, col;
+                place(q, b0, r0, row, col);
+                if (!TURNED && row >= ext) row = ext - 1;
+                if (TURNED && col >= ext) col = b0;
+                __builtin_memcpy(&r[q], base + row * ld + col, 16);
+            }
+            return;
+        }
 #pragma unroll
         for (int q = 0; q < NC; ++q) {
             int64_t row, col;
@@ -315,7 +336,7 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
     KeepBits<V> keep;
 
     __device__ __forceinline__ void load(const GemmArgs& A, int64_t b0, int64_t ext, int64_t r0, int64_t rend) {
-        S::load((const T*)A.P, A.ldp, b0, ext, r0, rend);
+        S::load((const T*)A.P, A.ldp, b0, ext, r0, rend, A.R);
         if (!A.dz.z) return;
         const bool relu = A.dz.act == PSFM_ACT_RELU;
 #pragma unroll
@@ -527,8 +548,8 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
             if constexpr (DZ)
                 sp.load(A, i0, A.I, r, rend);
             else
-                sp.load(P, A.ldp, i0, A.I, r, rend);
-            sq.load(Q, A.ldq, j0, A.J, r, rend);
+                sp.load(P, A.ldp, i0, A.I, r, rend, A.R);
+            sq.load(Q, A.ldq, j0, A.J, r, rend, A.R);
         }
     };
     auto put = [&](lds8* lds, int64_t r) {
