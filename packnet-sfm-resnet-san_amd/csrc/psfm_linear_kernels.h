@@ -217,12 +217,12 @@ __device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& ke
 // ---- LDS images ----------------------------------------------------------------------------
 // Straight operand: one 128-byte row of reduction per output row; its eight 16-byte chunks are XORed by the
 // row so that 16 lanes reading the same chunk of 16 rows hit 16 bank quads.  Turned operand: one row per
-// reduction index, chunks XORed so that the transposing reads (16 bits: 4 rows x 32 bytes a 16-lane group;
-// 32 bits: 64 bytes a group, 4 groups 4 rows apart) spread over the banks.
+// reduction index, chunks XORed so that the reads (16 bits: transposing, 4 rows x 32 bytes a 16-lane group;
+// 32 bits: 128 or 256 bytes of a row a group, the groups 4 rows apart) spread over the banks.
 __device__ __forceinline__ int swz_straight(int row) { return (row >> 1) & 7; }
 template <typename T, int B>
 __device__ __forceinline__ int swz_turned(int row) {
-    if (sizeof(T) == 4) return ((row >> 2) & 3) << 2;
+    if (sizeof(T) == 4) return (((row >> 2) & 1) << 3) | (((row >> 3) & 1) << 2);
     if (B == 64) return (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) << 1;
     return ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
 }
@@ -407,16 +407,8 @@ __device__ __forceinline__ u4v fragment(const lds8* lds, int b, int ks) {
         const int row = b + n;
         return *(const PSFM_LDS u4v*)(lds + row * 128 + (((ks * 4 + g) ^ swz_straight(row)) << 4));
     }
-    constexpr int RB = B * (int)sizeof(T);
-    if constexpr (sizeof(T) == 4) {
-        u4v v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = ks * 16 + 4 * g + i, ch = (b >> 2) + (n >> 2);
-            v[i] = *(const PSFM_LDS uint32_t*)(lds + row * RB + ((ch ^ swz_turned<T, B>(row)) << 4) + 4 * (n & 3));
-        }
-        return v;
-    } else {
+    if constexpr (sizeof(T) == 2) {
+        constexpr int RB = B * 2;
         // a 16-lane group reads 4 rows x 16 values, lane n gets column n of the 4 rows
         typedef PSFM_LDS s4 lds_s4;
         const int ch = (b >> 3) + ((n & 3) >> 1), r0 = ks * 32 + 8 * g + (n >> 2), r1 = r0 + 4;
@@ -426,6 +418,23 @@ __device__ __forceinline__ u4v fragment(const lds8* lds, int b, int ks) {
             (lds_s4*)(lds + r1 * RB + ((ch ^ swz_turned<T, B>(r1)) << 4) + 8 * (n & 1)));
         typedef short s8 __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(u4v, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    }
+    __builtin_unreachable();   // turned 32-bit operands: fragments_turned32
+}
+
+// S of them of a turned 32-bit operand.  Lane n takes the S neighbouring output rows b + S n + s of each reduction
+// index, one read of 4 S bytes, so operand s holds every S-th output row: `product` puts the results in order.
+template <int S, int B, int ks>
+__device__ __forceinline__ void fragments_turned32(const lds8* lds, int b, u4v (&f)[S]) {
+    static_assert(S == 2 || S == 4, "a read of 8 or 16 bytes");
+    typedef unsigned int uSv __attribute__((ext_vector_type(S)));
+    const int l = threadIdx.x & 63, g = l >> 4, col = b + S * (l & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = ks * 16 + 4 * g + i;
+        const uSv v = *(const PSFM_LDS uSv*)(lds + row * B * 4 + (((col >> 2) ^ swz_turned<float, B>(row)) << 4) + 4 * (col & 3));
+#pragma unroll
+        for (int s = 0; s < S; ++s) f[s][i] = v[s];
     }
 }
 
@@ -474,7 +483,9 @@ __device__ __forceinline__ void fragments_turned(const lds8* lds, int b, u4v (&f
 // The S operands of a wave's step.
 template <typename T, int S, int B, bool TURNED, bool DMA, int ks>
 __device__ __forceinline__ void fragments(const lds8* lds, int b, u4v (&f)[S]) {
-    if constexpr (TURNED && DMA && sizeof(T) == 2) {
+    if constexpr (TURNED && sizeof(T) == 4) {
+        fragments_turned32<S, B, ks>(lds, b, f);
+    } else if constexpr (TURNED && DMA) {
         fragments_turned<S, B, ks>(lds, b, f);
     } else {
 #pragma unroll
@@ -620,16 +631,29 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
         }
     }
 
+    // A lane holds row row_of(a) and, for q = 0 .. SJ - 1, the columns col_of(q) .. + 3 of it (fragments_turned32: every SJ-th
+    // or SI-th is its operand's).
     const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
+    constexpr bool ROWS32 = PT && sizeof(T) == 4, COLS32 = QT && sizeof(T) == 4;
+    auto row_of = [&](int a) { return wi * (BI / WI) + (ROWS32 ? SI * n + a : 16 * a + n); };
+    auto col_of = [&](int q) { return wj * (BJ / WJ) + (COLS32 ? 4 * SJ * g + 4 * q : 16 * q + 4 * g); };
+    auto four = [&](int a, int q) {
+        if constexpr (!COLS32) return acc[a][q];
+        f4 v;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = acc[a][(4 * q + t) % SJ][(4 * q + t) / SJ];
+        return v;
+    };
     if (A.splits > 1) {
 #pragma unroll
         for (int a = 0; a < SI; ++a) {
-            const int64_t i = i0 + wi * (BI / WI) + a * 16 + n;
+            const int64_t i = i0 + row_of(a);
 #pragma unroll
-            for (int b = 0; b < SJ; ++b) {
-                const int64_t j = j0 + wj * (BJ / WJ) + b * 16 + 4 * g;
+            for (int q = 0; q < SJ; ++q) {
+                const int64_t j = j0 + col_of(q);
                 if (i >= A.I || j >= A.J) continue;
-                const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+                const f4 x = four(a, q);
+                const float v[4] = {x[0], x[1], x[2], x[3]};
                 store_run(A.part + (split * A.I + i) * A.J + j, v, A.J - j < 4 ? (int)(A.J - j) : 4);
             }
         }
@@ -654,13 +678,11 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
         if (band) __syncthreads();
 #pragma unroll
         for (int a = 0; a < SI; ++a) {
-            const int first = wi * (BI / WI) + a * 16 - band * BAND;
-            if (first < 0 || first >= BAND) continue;
+            const int i = row_of(a) - band * BAND;
+            if (i < 0 || i >= BAND) continue;
 #pragma unroll
-            for (int b = 0; b < SJ; ++b) {
-                const int c = (wj * (BJ / WJ) + b * 16) / 4 + g;
-                *reinterpret_cast<f4*>(tile + (first + n) * BJ + ((c ^ n) << 2)) = acc[a][b];
-            }
+            for (int q = 0; q < SJ; ++q)
+                *reinterpret_cast<f4*>(tile + i * BJ + (((col_of(q) >> 2) ^ (i & 15)) << 2)) = four(a, q);
         }
         __syncthreads();
         const int64_t ib = i0 + band * BAND;
