@@ -58,27 +58,40 @@ struct Plan {
     int64_t blocks() const { return ti * tj * splits; }
 };
 
-// Tiles: the largest that still fills the 256 CUs and computes at most an eighth more than the smallest
-// would (a 64-column layer in 256-column tiles: 86 us, 42 in 128), else the smallest.  A long reduction is split while
-// that leaves every CU fewer than `fill` / 256 workgroups and a split keeps eight LDS stages, four where the tiles
-// alone leave CUs idle.
-Plan plan(int dtype, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1, int64_t fill = 768) {
-    Plan p{0, 0, 0, 0, 1};
-    const Tile& t0 = LINEAR_TILES[0];
-    const double least = (double)(up(I, t0.bi) * t0.bi) * (double)(up(J, t0.bj) * t0.bj);
-    for (int v = std::min(largest, dtype == PSFM_DTYPE_F32 ? 1 : 2); v >= 0; --v) {
-        const Tile& t = LINEAR_TILES[v];
-        p.variant = v, p.ti = up(I, t.bi), p.tj = up(J, t.bj);
-        if (p.ti * p.tj >= 256 && (double)(p.ti * t.bi) * (double)(p.tj * t.bj) <= 1.125 * least) break;
+// The tile and the splits of the reduction that should take least time, from what a stage of 128 bytes of reduction
+// takes (us): `alone` where a CU has one workgroup and waits for memory, `busy` per workgroup where it
+// has enough of them; splits add a launch and their way through memory.  Sizes from 256 x 4096 x 1024 to
+// 16384 x 1024 x 256 were timed with every tile and 1 .. 16 splits; the choice is within a tenth of the best one
+// (bf16 1024 x 1024 x 1024: 10.0 us as chosen, 64 tiles in one piece; two pieces 13.7; 128 tiles 16.7; 256 tiles 33.6.
+// 1024 x 1024 over 4096: 23.1 in three pieces, 36 in one.  512 x 4096 over 4096: 32.0, 128 tiles in four pieces).  Rows
+// that are no whole chunks go through registers, and wait for memory half as long again (1531 x 517 x 771: 17.7 us
+// in two pieces, 15.5 in one).
+struct TileTime {
+    double alone, busy;
+};
+constexpr TileTime TIMES16[] = {{0.55, 0.22}, {1.0, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}};
+
+Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1) {
+    static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512};
+    const bool wide = d->dtype == PSFM_DTYPE_F32;
+    const TileTime* times = wide ? TIMES32 : TIMES16;
+    const int64_t stage = 128 / size_of(d->dtype), stages = up(R, stage), v16 = 16 / size_of(d->dtype);
+    const double wait = d->N % v16 || d->K % v16 || d->ldx % v16 ? 1.5 : 1.0;
+    Plan best{0, 0, 0, 0, 1};
+    double least = 0;
+    for (int v = std::min(largest, wide ? 1 : 2); v >= 0; --v) {
+        const int64_t ti = up(I, LINEAR_TILES[v].bi), tj = up(J, LINEAR_TILES[v].bj);
+        for (const int want : SPLITS) {
+            const int64_t per = std::max<int64_t>(1, up(stages, want)), n = std::max<int64_t>(1, up(stages, per));
+            if (want > 1 && (per < 2 || ti * tj * n > 4096)) break;
+            const double blocks = (double)ti * (double)tj * (double)n, load = std::min(1.0, blocks / 512);
+            double t = (double)per * std::max(times[v].alone * wait * (0.64 + 0.36 * load),
+                                              times[v].busy * (double)up((int64_t)std::min(blocks, 1e15), 256));
+            if (n > 1) t += 4.0 + 0.012 * (double)n + (double)n * (double)I * (double)J * 8 / 3e6;
+            if (best.rsplit == 0 || t < least) least = t, best = Plan{v, ti, tj, per * stage, (int)n};
+        }
     }
-    const int64_t stage = 128 / size_of(dtype), stages = up(R, stage), tiles = p.ti * p.tj;
-    int64_t splits = 1;
-    if (tiles > 0 && p.variant == 0)
-        splits = std::max<int64_t>(1, std::min(tiles < 256 ? up(fill, tiles) : fill / tiles, stages / (tiles < 256 ? 4 : 8)));
-    const int64_t per = std::max<int64_t>(1, up(stages, splits));
-    p.rsplit = per * stage;
-    p.splits = (int)std::max<int64_t>(1, up(stages, per));
-    return p;
+    return best;
 }
 
 int64_t part_bytes(const Plan& p, int64_t I, int64_t J) { return p.splits > 1 ? p.splits * I * J * 4 : 0; }
@@ -126,8 +139,8 @@ BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db)
     const bool cheap = columns <= 4 || (double)columns * (double)d->M * (double)d->N < 8e6;
     b.stage = any && (b.dx || b.dw) && cheap && (make || (want_db && b.dw));
     const int largest = b.stage ? 0 : LINEAR_NTILES - 1;
-    if (b.dx) b.pdx = plan(d->dtype, d->M, d->K, d->N, largest);
-    if (b.dw) b.pdw = plan(d->dtype, d->N, d->K, d->M, largest, b.dx ? 256 : 768);
+    if (b.dx) b.pdx = plan(d, d->M, d->K, d->N, largest);
+    if (b.dw) b.pdw = plan(d, d->N, d->K, d->M, largest);
     b.pass = any && !b.stage && ((make && (b.dx || b.dw)) || want_db);
     if (b.stage && want_db && !b.dw) b.pass = true;      // the column sums alone
     b.dz = b.pass && !b.stage && make && (b.dx || b.dw);
@@ -150,7 +163,7 @@ extern "C" {
 
 int64_t psfm_linear_fwd_ws_bytes(const psfm_linear* d) {
     if (check(d)) return -1;
-    return skinny(d) ? 0 : part_bytes(plan(d->dtype, d->M, d->N, d->K), d->M, d->N);
+    return skinny(d) ? 0 : part_bytes(plan(d, d->M, d->N, d->K), d->M, d->N);
 }
 
 int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const void* bias, const void* res, void* y,
@@ -168,7 +181,7 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
         if (up(d->N, 16) > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more columns than a launch holds");
         return status(o.skinny(vec, SkinnyArgs{x, w, d->ldx, d->M, d->N, d->K, e}, s), "psfm_linear_fwd: launch");
     }
-    const Plan p = plan(d->dtype, d->M, d->N, d->K);
+    const Plan p = plan(d, d->M, d->N, d->K);
     if (p.splits > 1 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
     if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more tiles than a launch holds");
     GemmArgs a{};
