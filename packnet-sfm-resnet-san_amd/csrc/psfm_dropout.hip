@@ -7,6 +7,7 @@
 // workgroup finds its first row and the threads go on in 32 bits.
 #include "../../include/psfm_dropout.h"
 
+#include <algorithm>
 #include <string>
 
 #include "psfm_philox.h"
@@ -119,8 +120,8 @@ extern "C" {
 int psfm_dropout(const void* x, int64_t ldx, const void* res, int64_t ldr, int dtype, int64_t rows, int64_t cols,
                  int64_t mask_rows, double p, const int64_t* rng, void* y, void* stream) {
     const int64_t most = (int64_t)1 << 40;
-    if (rows < 0 || cols < 0 || rows > most || cols > most || (double)rows * (double)cols > 1e18)
-        return fail(-1, "psfm_dropout: rows and cols must be 0 .. 2^40");
+    if (rows < 0 || cols < 0 || rows > most || cols > most || (double)rows * (double)std::max({cols, ldx, ldr}) > 1e18)
+        return fail(-1, "psfm_dropout: rows and cols must be 0 .. 2^40, the whole below 10^18 values");
     if (dtype != PSFM_DTYPE_F32 && dtype != PSFM_DTYPE_F16 && dtype != PSFM_DTYPE_BF16)
         return fail(-2, "psfm_dropout: dtype must be PSFM_DTYPE_F32 / F16 / BF16");
     if (!(p >= 0.0 && p <= 1.0)) return fail(-3, "psfm_dropout: p must be in 0 .. 1");

@@ -127,7 +127,10 @@ class CounterDropout(nn.Module):
     """Dropout whose masks are (seed, offset), the offset counted on the device: in training every forward draws
     the next one, also in a captured graph's replays.  The ranks of a data-parallel job, which hold the same
     buffers, take seed + rank; the layers of one network take different first offsets.  The state is no part
-    of the state_dict: checkpoints of networks with nn.Dropout load as they are."""
+    of the state_dict: checkpoints of networks with nn.Dropout load as they are.
+
+    A forward that is run again for its backward (activation checkpointing) would draw another mask: draw() before
+    it, and give the Drop to dropout or linear_act inside."""
 
     def __init__(self, p, seed, offset=0, channels=False):
         super().__init__()

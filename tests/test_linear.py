@@ -110,7 +110,7 @@ def drop_and_keep(M, N, p, dev, share=1, seed=77):
 # reductions that are split; every direction has its long one
 SIZES = [(1, 1, 1), (1, 512, 512), (2, 33, 1031), (5, 17, 33), (16, 64, 4096), (17, 1030, 64), (64, 64, 64),
          (65, 63, 66), (130, 257, 129), (128, 128, 32), (127, 256, 40), (1000, 64, 32), (300, 2056, 72), (4099, 24, 48),
-         (9001, 13, 7), (2500, 320, 264)]
+         (9001, 13, 7), (2500, 320, 264), (70001, 3, 5), (6000, 1, 70)]
 
 
 @gpu
@@ -294,7 +294,7 @@ def test_everything_dropped(dev, dtype):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_empty_sizes(dev, dtype):
-    for M, N, K in ((0, 8, 16), (8, 0, 16), (8, 16, 0), (0, 0, 0)):
+    for M, N, K in ((0, 8, 16), (8, 0, 16), (8, 16, 0), (0, 0, 0), (100, 16, 0), (0, 100, 200), (200, 0, 64)):
         t = make(M, N, K, dtype, dev, 1, True, True)
         y = linear_act(t["x"], t["w"], t["bias"], LI.ACT_SILU, t["res"], Drop(0.5, pair(1, 1, dev)))
         dx, dw, db = torch.autograd.grad(y, [t["x"], t["w"], t["bias"]], t["dy"])
@@ -389,6 +389,40 @@ def test_captured_and_replayed_with_new_inputs(dev, M, N, K):
         for out in outs:
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+@gpu
+def test_second_derivatives_are_refused(dev):
+    """A gradient with a graph of its own has the right values and raises when that graph is differentiated; the residual's,
+    which is dy itself, goes on being differentiable."""
+    t = make(40, 24, 16, torch.float32, dev, 1, True, True)
+    names = ("x", "w", "bias", "res")
+    for drop in (None, Drop(0.5, pair(1, 1, dev))):
+        for f in (lambda: linear_act(t["x"], t["w"], t["bias"], LI.ACT_SILU, t["res"], drop),
+                  lambda: dropout(t["res"], drop or Drop(0.1, pair(2, 2, dev)), t["res"])):
+            leaves = [t[k] for k in names]
+            dy = t["dy"].clone().requires_grad_(True)
+            once = torch.autograd.grad(f(), leaves, dy, allow_unused=True)
+            graph = torch.autograd.grad(f(), leaves, dy, create_graph=True, allow_unused=True)
+            assert all(a is None or torch.equal(a, b) for a, b in zip(once, graph))
+            for g in graph:
+                if g is not None and g is not graph[3]:
+                    with pytest.raises(RuntimeError, match="differentiated twice"):
+                        g.sum().backward(retain_graph=True)
+    dy = t["dy"].clone().requires_grad_(True)
+    g, = torch.autograd.grad(linear_act(t["x"], t["w"], residual=t["res"]), t["res"], dy, create_graph=True)
+    assert torch.equal(torch.autograd.grad((g * g).sum(), dy)[0], 2 * dy)
+
+
+@gpu
+def test_saved_tensors_changed_in_place_are_refused(dev):
+    for change, act in (("x", LI.ACT_NONE), ("w", LI.ACT_NONE), ("y", LI.ACT_RELU)):
+        t = make(40, 24, 16, torch.bfloat16, dev, 1, False)
+        y = linear_act(t["x"], t["w"], None, act)
+        with torch.no_grad():
+            (y if change == "y" else t[change]).mul_(2)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(y, [t["x"], t["w"]], t["dy"])
 
 
 @gpu
