@@ -87,7 +87,7 @@ Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = L
             const double blocks = (double)ti * (double)tj * (double)n, load = std::min(1.0, blocks / 512);
             double t = (double)per * std::max(times[v].alone * wait * (0.64 + 0.36 * load),
                                               times[v].busy * (double)up((int64_t)std::min(blocks, 1e15), 256));
-            if (n > 1) t += 4.0 + 0.012 * (double)n + (double)n * (double)I * (double)J * 8 / 3e6;
+            if (n > 1) t += 4.0 + 0.15 * (double)std::min<int64_t>(n, 8) + 0.012 * (double)n + (double)n * (double)I * (double)J * 8 / 5e6;
             if (best.rsplit == 0 || t < least) least = t, best = Plan{v, ti, tj, per * stage, (int)n};
         }
     }

@@ -514,11 +514,19 @@ __device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
     return x * per + (x < more ? x : more) + k;
 }
 
-// Tile `id` of `count` of a product.  WI x WJ waves.  The two stages are two objects, and the loop is written out for
-// both, so that the compiler sees that the reads of one do not wait for the loads into the other.
-template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, bool VEC, bool FULL, bool DZ>
+// Stages in LDS.  Two; three of the smallest tile where loads go into LDS and the reduction is long (DEEP), so that two
+// are on their way while one is multiplied: a CU with few workgroups waits for memory (4096 x 512 x 2048 bf16: 21.2 us
+// with two, 15.9 with three; 512 x 4096 x 4096: 38.8, 32.5).  Short ones live from workgroups a CU instead (184320 x
+// 64 x 32: 21 us with two and five a CU, 23.4 with three and three a CU).
+constexpr int DEEP_STAGES = 5;   // of reduction, at least
+template <bool DMA, bool DEEP>
+constexpr int STAGES = DMA && DEEP ? 3 : 2;
+
+// Tile `id` of `count` of a product.  WI x WJ waves.  The stages are objects of their own, and the loop is written out for
+// them, so that the compiler sees that the reads of one do not wait for the loads into another.
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, bool VEC, bool FULL, bool DZ, bool DEEP>
 __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t count,
-                                        uint8_t (&stage0)[(BI + BJ) * 128], uint8_t (&stage1)[(BI + BJ) * 128]) {
+                                        uint8_t (&stage0)[(BI + BJ) * 128], lds8* s1, lds8* s2) {
     constexpr int NTH = 64 * WI * WJ, BR = 128 / (int)sizeof(T), SI = BI / WI / 16, SJ = BJ / WJ / 16, V = CHUNK<T>;
     constexpr bool DMA = VEC && !DZ;
     const uint32_t tiles = A.ti * A.tj, w = xcd_run(id, count), split = w / tiles, t = w - split * tiles;
@@ -572,10 +580,6 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
             sq.store(lds + BI * 128);
         }
     };
-    auto ready = [&]() {   // this wave's loads into LDS have landed, and so have the others' behind the barrier
-        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-    };
     auto multiply_step = [&](const lds8* lp, auto ks) {
         u4v fp[SI], fq[SJ];
         fragments<T, SJ, BJ, QT, DMA, ks.value>(lp + BI * 128, wj * (BJ / WJ), fq);
@@ -589,25 +593,75 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
         multiply_step(lp, std::integral_constant<int, 0>());
         multiply_step(lp, std::integral_constant<int, 1>());
     };
-    // the stage that is filled: its last readers passed the barrier before this step
-    auto step = [&](const lds8* now, lds8* next, int k) {
-        const bool more = k + 1 < nk;
-        const int64_t r = r0 + (int64_t)(k + 1) * BR;
-        if (more) fetch(next, r);
-        multiply(now);
-        if (more) put(next, r);
-        ready();
-    };
     lds8* const s0 = (lds8*)&stage0[0];
-    lds8* const s1 = (lds8*)&stage1[0];
-    if (nk > 0) {
-        fetch(s0, r0);
-        put(s0, r0);
-    }
-    ready();
-    for (int k = 0; k < nk; k += 2) {
-        step(s0, s1, k);
-        if (k + 1 < nk) step(s1, s0, k + 1);
+    if constexpr (DMA) {
+        constexpr int NST = STAGES<true, DEEP>, LOADS = SP::NC + SQ::NC;
+        constexpr int WAIT_ALL = 0x70;   // s_waitcnt's vmcnt and lgkmcnt at 0 (vmcnt: the low four bits), expcnt at its top
+        static_assert(NST == 2 || LOADS < 16, "vmcnt's low bits");
+        lds8* const st[3] = {s0, s1, s2};
+        // Behind the barrier stage k has landed, for every wave, and the one before it has been read, so that the next but
+        // one can be loaded over it.  The barrier is bare: a fence would wait for all loads.
+        auto step = [&](auto i, int k) {
+            asm volatile("" ::: "memory");
+            if (NST == 3 && k + 1 < nk)
+                __builtin_amdgcn_s_waitcnt(WAIT_ALL | LOADS);   // stage k + 1 may be on its way
+            else
+                __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (k + NST - 1 < nk) fetch(st[(i.value + NST - 1) % NST], r0 + (int64_t)(k + NST - 1) * BR);
+            multiply(st[i.value]);
+        };
+        // the same with a stage to load for certain: then the compiler can tell that the older loads have landed
+        auto step_on = [&](auto i, int k) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(WAIT_ALL | LOADS);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            fetch(st[(i.value + 2) % 3], r0 + (int64_t)(k + 2) * BR);
+            multiply(st[i.value]);
+        };
+        int k = 0;
+        if (NST == 3 && nk > 4) {
+            fetch(st[0], r0);
+            fetch(st[1], r0 + BR);
+            do {
+                step_on(std::integral_constant<int, 0>(), k);
+                step_on(std::integral_constant<int, 1>(), k + 1);
+                step_on(std::integral_constant<int, 2>(), k + 2);
+                k += 3;
+            } while (k + 4 < nk);
+        } else {
+#pragma unroll
+            for (int q = 0; q < NST - 1; ++q)
+                if (q < nk) fetch(st[q], r0 + (int64_t)q * BR);
+        }
+        for (; k < nk; k += NST) {
+            step(std::integral_constant<int, 0>(), k);
+            if (k + 1 < nk) step(std::integral_constant<int, 1>(), k + 1);
+            if constexpr (NST == 3)
+                if (k + 2 < nk) step(std::integral_constant<int, 2>(), k + 2);
+        }
+        __syncthreads();
+    } else {
+        // the stage that is filled: its last readers passed the barrier before this step
+        auto step = [&](const lds8* now, lds8* next, int k) {
+            const bool more = k + 1 < nk;
+            const int64_t r = r0 + (int64_t)(k + 1) * BR;
+            if (more) fetch(next, r);
+            multiply(now);
+            if (more) put(next, r);
+            __syncthreads();
+        };
+        if (nk > 0) {
+            fetch(s0, r0);
+            put(s0, r0);
+        }
+        __syncthreads();
+        for (int k = 0; k < nk; k += 2) {
+            step(s0, s1, k);
+            if (k + 1 < nk) step(s1, s0, k + 1);
+        }
     }
 
     if constexpr (DZ && PT) {
@@ -702,20 +756,27 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     }
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool VEC>
+#define PSFM_STAGES(DMA)                                                                                 \
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128],    \
+        stage2[STAGES<DMA, DEEP> == 3 ? (BI + BJ) * 128 : 16];                                           \
+    lds8* const s1 = (lds8*)&stage1[0];                                                                  \
+    lds8* const s2 = (lds8*)&stage2[0];
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DEEP>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_forward(const GemmArgs A) {
-    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128];
-    product<T, BI, BJ, WI, WJ, false, false, VEC, true, false>(A, blockIdx.x, gridDim.x, stage0, stage1);
+    PSFM_STAGES(VEC)
+    product<T, BI, BJ, WI, WJ, false, false, VEC, true, false, DEEP>(A, blockIdx.x, gridDim.x, stage0, s1, s2);
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DZ>
+template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DZ, bool DEEP>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_pair(const PairArgs A) {
-    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128];
+    PSFM_STAGES(VEC && !DZ)
     if (blockIdx.x < A.ndw)
-        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ>(A.dw, blockIdx.x, A.ndw, stage0, stage1);
+        product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ, DEEP>(A.dw, blockIdx.x, A.ndw, stage0, s1, s2);
     else
-        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ>(A.dx, blockIdx.x - A.ndw, A.ndx, stage0, stage1);
+        product<T, BI, BJ, WI, WJ, false, true, VEC, false, DZ, DEEP>(A.dx, blockIdx.x - A.ndw, A.ndx, stage0, s1, s2);
 }
+#undef PSFM_STAGES
 
 // y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction, 128 bytes of each row (two steps) a
 // turn; each reads 16 rows of W straight into the matrix instructions' operands, U steps in flight, and x's few rows
@@ -900,43 +961,52 @@ __global__ __launch_bounds__(DZ_THREADS) void k_dz(const DzPassArgs A) {
 }
 
 // ---- launches --------------------------------------------------------------------------------
-template <typename T, int BI, int BJ, int WI, int WJ>
+template <typename T>
+bool deep(const GemmArgs& a) {
+    return a.rsplit >= DEEP_STAGES * (128 / (int64_t)sizeof(T)) && a.R >= DEEP_STAGES * (128 / (int64_t)sizeof(T));
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool DEEP>
 void launch_forward(bool vec, const GemmArgs& a, hipStream_t s) {
     if (vec)
-        k_forward<T, BI, BJ, WI, WJ, true><<<dim3(a.blocks()), 64 * WI * WJ, 0, s>>>(a);
+        k_forward<T, BI, BJ, WI, WJ, true, DEEP><<<dim3(a.blocks()), 64 * WI * WJ, 0, s>>>(a);
     else
-        k_forward<T, BI, BJ, WI, WJ, false><<<dim3(a.blocks()), 64 * WI * WJ, 0, s>>>(a);
+        k_forward<T, BI, BJ, WI, WJ, false, false><<<dim3(a.blocks()), 64 * WI * WJ, 0, s>>>(a);
 }
 template <typename T>
 int forward_of(int variant, bool vec, const GemmArgs& a, hipStream_t s) {
-    if (variant == 0)
-        launch_forward<T, 64, 64, 2, 2>(vec, a, s);
+    if (variant == 0 && deep<T>(a))
+        launch_forward<T, 64, 64, 2, 2, true>(vec, a, s);
+    else if (variant == 0)
+        launch_forward<T, 64, 64, 2, 2, false>(vec, a, s);
     else if (variant == 1 || sizeof(T) == 4)
-        launch_forward<T, 128, 128, 2, 2>(vec, a, s);
+        launch_forward<T, 128, 128, 2, 2, false>(vec, a, s);
     else if constexpr (sizeof(T) == 2)
-        launch_forward<T, 256, 256, 2, 4>(vec, a, s);
+        launch_forward<T, 256, 256, 2, 4, false>(vec, a, s);
     return (int)hipGetLastError();
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool DZ>
+template <typename T, int BI, int BJ, int WI, int WJ, bool DZ, bool DEEP>
 void launch_pair(bool vec, const PairArgs& a, hipStream_t s) {
     const dim3 grid(a.ndx + a.ndw), block(64 * WI * WJ);
     if (vec)
-        k_pair<T, BI, BJ, WI, WJ, true, DZ><<<grid, block, 0, s>>>(a);
+        k_pair<T, BI, BJ, WI, WJ, true, DZ, DEEP><<<grid, block, 0, s>>>(a);
     else
-        k_pair<T, BI, BJ, WI, WJ, false, DZ><<<grid, block, 0, s>>>(a);
+        k_pair<T, BI, BJ, WI, WJ, false, DZ, false><<<grid, block, 0, s>>>(a);
 }
 // dz is made on the way only in the smallest tiles: the others have no registers left for it
 template <typename T>
 int pair_of(int variant, bool vec, bool dz, const PairArgs& a, hipStream_t s) {
     if (variant == 0 && dz)
-        launch_pair<T, 64, 64, 2, 2, true>(vec, a, s);
+        launch_pair<T, 64, 64, 2, 2, true, false>(vec, a, s);
+    else if (variant == 0 && (a.ndx == 0 || deep<T>(a.dx)) && (a.ndw == 0 || deep<T>(a.dw)))
+        launch_pair<T, 64, 64, 2, 2, false, true>(vec, a, s);
     else if (variant == 0)
-        launch_pair<T, 64, 64, 2, 2, false>(vec, a, s);
+        launch_pair<T, 64, 64, 2, 2, false, false>(vec, a, s);
     else if (variant == 1 || sizeof(T) == 4)
-        launch_pair<T, 128, 128, 2, 2, false>(vec, a, s);
+        launch_pair<T, 128, 128, 2, 2, false, false>(vec, a, s);
     else if constexpr (sizeof(T) == 2)
-        launch_pair<T, 256, 256, 2, 4, false>(vec, a, s);
+        launch_pair<T, 256, 256, 2, 4, false, false>(vec, a, s);
     return (int)hipGetLastError();
 }
 
