@@ -59,17 +59,16 @@ struct Plan {
 };
 
 // The tile and the splits of the reduction that should take least time, from what a stage of 128 bytes of reduction
-// takes (us): `alone` where a CU has one workgroup and waits for memory, `busy` per workgroup where it
-// has enough of them; splits add a launch and their way through memory.  Sizes from 256 x 4096 x 1024 to
-// 16384 x 1024 x 256 were timed with every tile and 1 .. 16 splits; the choice is within a tenth of the best one
-// (bf16 1024 x 1024 x 1024: 10.0 us as chosen, 64 tiles in one piece; two pieces 13.7; 128 tiles 16.7; 256 tiles 33.6.
-// 1024 x 1024 over 4096: 23.1 in three pieces, 36 in one.  512 x 4096 over 4096: 32.0, 128 tiles in four pieces).  Rows
-// that are no whole chunks go through registers, and wait for memory half as long again (1531 x 517 x 771: 17.7 us
-// in two pieces, 15.5 in one).
+// takes (us): `alone` where a CU has one or two workgroups and waits for memory, `busy` per workgroup where it
+// has enough of them; splits add a launch and their way through memory.  From a sweep of every tile and 1 .. 16
+// splits over products from 300 x 500 x 1200 to 16384 x 1024 x 256 (I x J x R); the choice was within a seventh of the best
+// one (bf16 1024 x 1024 x 1024: 8.0 us as chosen, 64 tiles in one piece; two pieces 13.8; 128 tiles 16.7; 256 tiles 33.
+// 256 x 1024 x 4096: 11.1 in four pieces, 12.2 in two.  512 x 4096 x 4096: 26.9, 128 tiles in four pieces 31.3).  Rows that
+// are no whole chunks go through registers, and wait for memory half as long again.
 struct TileTime {
     double alone, busy;
 };
-constexpr TileTime TIMES16[] = {{0.55, 0.22}, {1.0, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}};
+constexpr TileTime TIMES16[] = {{0.42, 0.22}, {1.15, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}};
 
 Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1) {
     static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512};
