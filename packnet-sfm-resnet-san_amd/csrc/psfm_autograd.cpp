@@ -106,6 +106,19 @@ void refuse_foreign_capture() {
     TORCH_CHECK(false, msg);
 }
 
+// A captured backward accumulates into a leaf on the stream that the leaf's accumulator is bound to, and an accumulator
+// lives as long as any graph of its leaf does.  One left from eager work on the default stream cannot take part in a
+// capture (the process ends in capture_end), so the forward is refused.
+void refuse_bound_leaf(const at::Tensor& t) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    const std::optional<c10::Stream> s = accumulator ? accumulator->stream() : std::nullopt;
+    TORCH_CHECK(!s || s->id() != 0,
+                "psfm: a HIP-graph capture is in progress and a graph from eager work on the default stream still holds one "
+                "of this call's leaves, whose gradient a captured backward would accumulate on that stream.  Free the "
+                "outputs of that work first (or run it on a side stream)");
+}
+
 // ---- tensors -------------------------------------------------------------------------------------
 void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -234,7 +247,10 @@ at::Tensor linear_act(const at::Tensor& x_, const at::Tensor& weight_, const std
                      rng = rng_.value_or(at::Tensor());
     const bool grad_x = wants(x_), grad_w = wants(weight_), grad_b = wants(bias_in);
     std::shared_ptr<LinearActBackward> node;
+    const bool in_capture = capturing();
     if (at::GradMode::is_enabled() && (grad_x || grad_w || grad_b || wants(res_in))) {
+        if (in_capture)
+            for (const at::Tensor& t : {x_, weight_, bias_in, res_in}) refuse_bound_leaf(t);
         node = std::shared_ptr<LinearActBackward>(new LinearActBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x_, weight_, bias_in, res_in));
     }
@@ -264,7 +280,7 @@ at::Tensor linear_act(const at::Tensor& x_, const at::Tensor& weight_, const std
         TORCH_CHECK(n >= 0, "psfm_linear_fwd_ws_bytes failed: ", entry.linear_error());
         const at::Tensor work = workspace(n, x);
         void* stream = stream_of(x);
-        if (node && !capturing()) node->live.ran_forward((uintptr_t)stream);
+        if (node && !in_capture) node->live.ran_forward((uintptr_t)stream);
         const int rc = entry.fwd(&d, at_of(x), at_of(weight), at_of(bias), at_of(res), at_of(y), at_of(z), at_of(work), stream);
         TORCH_CHECK(rc == 0, "psfm_linear_fwd failed (", rc, "): ", entry.linear_error());
     }
@@ -326,10 +342,13 @@ at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residua
     const int64_t share = mask_rows(x.sizes(), channels);
     std::shared_ptr<DropoutBackward> node;
     if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {
+        const bool in_capture = capturing();
+        if (in_capture)
+            for (const at::Tensor& t : {x, res}) refuse_bound_leaf(t);
         node = std::shared_ptr<DropoutBackward>(new DropoutBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, res));
         c10::DeviceGuard guard(x.device());
-        if (!capturing()) node->live.ran_forward((uintptr_t)stream_of(x));
+        if (!in_capture) node->live.ran_forward((uintptr_t)stream_of(x));
     }
     at::Tensor y = drop_launch(x, res, p, rng, share);
     if (node) {

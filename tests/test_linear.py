@@ -426,6 +426,33 @@ def test_saved_tensors_changed_in_place_are_refused(dev):
 
 
 @gpu
+def test_capture_with_a_leaf_that_an_eager_graph_holds_is_refused(dev):
+    """Whichever operator made that graph: the leaf's accumulator is bound to the default stream.  Freed, the same
+    capture goes ahead."""
+    t = make(40, 24, 16, torch.float32, dev, 1)
+    held = torch.nn.functional.linear(t["x"], t["w"], t["bias"])
+    torch.autograd.grad(held, t["w"], t["dy"], retain_graph=True)
+    drop, buf = Drop(0.5, pair(1, 1, dev)), torch.zeros(8, device=dev)
+    for call in (lambda: linear_act(t["x"], t["w"]), lambda: dropout(t["x"], drop)):
+        with pytest.raises(RuntimeError, match="still holds one of this call's leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                buf.add_(1)
+                call()
+        torch.cuda.synchronize()
+    del held
+    gc.collect()
+    want = torch.autograd.grad(linear_act(t["x"], t["w"], t["bias"]), [t["x"], t["w"]], t["dy"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(linear_act(t["x"], t["w"], t["bias"]), [t["x"], t["w"]], t["dy"])
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
 def test_streams_side_by_side(dev):
     """Calls on two streams at once have workspaces of their own."""
     ts = [make(300 + s, 96, 4096, torch.float16, dev, s, True, True) for s in range(2)]
