@@ -325,7 +325,10 @@ struct DmaStager {
 };
 
 // The same of dz, made from dy and z on the way to LDS, with the sums of this thread's columns (turned: they stay
-// the same in all its chunks) before dz is rounded to the type for the matrix cores.
+// the same in all its chunks) before dz is rounded to the type for the matrix cores.  16 bits: what that rounding leaves
+// goes to a second image and a second product, so that a gradient has one rounding and not two (few values are summed
+// here at times, and then the two showed: up to 1.6 times the error of one).  These products wait for memory,
+// not for the matrix cores.  No activation, or ReLU: dz is dy's own value or 0, and nothing is left.
 template <typename T, int B, int NTH, bool TURNED, bool VEC>
 struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
     using S = Stager<T, B, NTH, TURNED, VEC>;
@@ -357,7 +360,12 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
             }
         }
     }
-    __device__ __forceinline__ void store(lds8* lds, const GemmArgs& A, const PhiloxKey& key, int64_t b0, int64_t r0) {
+    static __device__ __forceinline__ bool has_rest(const GemmArgs& A) {
+        return sizeof(T) == 2 && A.dz.z && A.dz.act != PSFM_ACT_RELU;
+    }
+    // rest: the second image
+    __device__ __forceinline__ void store(lds8* lds, lds8* rest, const GemmArgs& A, const PhiloxKey& key, int64_t b0,
+                                          int64_t r0) {
         typedef T TV __attribute__((ext_vector_type(V)));
 #pragma unroll
         for (int q = 0; q < S::NC; ++q) {
@@ -394,6 +402,16 @@ struct DzStager : Stager<T, B, NTH, TURNED, VEC> {
                 if (TURNED) sum[k] += d[k];
             }
             S::put(lds, q, __builtin_bit_cast(u4v, o));
+            if constexpr (sizeof(T) == 2) {
+                if (has_rest(A)) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        const float high = (float)o[k];
+                        o[k] = (T)(fabsf(high) < INFINITY ? d[k] - high : 0.0f);   // nothing is left of an infinity
+                    }
+                    S::put(rest, q, __builtin_bit_cast(u4v, o));
+                }
+            }
         }
     }
 };
@@ -522,11 +540,15 @@ constexpr int DEEP_STAGES = 5;   // of reduction, at least
 template <bool DMA, bool DEEP>
 constexpr int STAGES = DMA && DEEP ? 3 : 2;
 
+// A stage's images: P, Q, and what dz's rounding left of P.
+template <typename T, int BI, int BJ, bool DZ>
+constexpr int STAGE_BYTES = (BI + BJ + (DZ && sizeof(T) == 2 ? BI : 0)) * 128;
+
 // Tile `id` of `count` of a product.  WI x WJ waves.  The stages are objects of their own, and the loop is written out for
 // them, so that the compiler sees that the reads of one do not wait for the loads into another.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, bool VEC, bool FULL, bool DZ, bool DEEP>
 __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t count,
-                                        uint8_t (&stage0)[(BI + BJ) * 128], lds8* s1, lds8* s2) {
+                                        uint8_t (&stage0)[STAGE_BYTES<T, BI, BJ, DZ>], lds8* s1, lds8* s2) {
     constexpr int NTH = 64 * WI * WJ, BR = 128 / (int)sizeof(T), SI = BI / WI / 16, SJ = BJ / WJ / 16, V = CHUNK<T>;
     constexpr bool DMA = VEC && !DZ;
     const uint32_t tiles = A.ti * A.tj, w = xcd_run(id, count), split = w / tiles, t = w - split * tiles;
@@ -574,12 +596,14 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     auto put = [&](lds8* lds, int64_t r) {
         if constexpr (!DMA) {
             if constexpr (DZ)
-                sp.store(lds, A, dkey, i0, r);
+                sp.store(lds, lds + (BI + BJ) * 128, A, dkey, i0, r);
             else
                 sp.store(lds);
             sq.store(lds + BI * 128);
         }
     };
+    bool has_rest = false;
+    if constexpr (DZ) has_rest = SP::has_rest(A);
     auto multiply_step = [&](const lds8* lp, auto ks) {
         u4v fp[SI], fq[SJ];
         fragments<T, SJ, BJ, QT, DMA, ks.value>(lp + BI * 128, wj * (BJ / WJ), fq);
@@ -588,6 +612,15 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
         for (int a = 0; a < SI; ++a)
 #pragma unroll
             for (int b = 0; b < SJ; ++b) acc[a][b] = mma<T>(fq[b], fp[a], acc[a][b]);
+        if constexpr (DZ && sizeof(T) == 2) {
+            if (has_rest) {
+                fragments<T, SI, BI, PT, DMA, ks.value>(lp + (BI + BJ) * 128, wi * (BI / WI), fp);
+#pragma unroll
+                for (int a = 0; a < SI; ++a)
+#pragma unroll
+                    for (int b = 0; b < SJ; ++b) acc[a][b] = mma<T>(fq[b], fp[a], acc[a][b]);
+            }
+        }
     };
     auto multiply = [&](const lds8* lp) {
         multiply_step(lp, std::integral_constant<int, 0>());
@@ -756,21 +789,21 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
     }
 }
 
-#define PSFM_STAGES(DMA)                                                                                 \
-    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BI + BJ) * 128], stage1[(BI + BJ) * 128],    \
-        stage2[STAGES<DMA, DEEP> == 3 ? (BI + BJ) * 128 : 16];                                           \
-    lds8* const s1 = (lds8*)&stage1[0];                                                                  \
+#define PSFM_STAGES(DMA, DZ)                                                                               \
+    constexpr int BYTES = STAGE_BYTES<T, BI, BJ, DZ>;                                                      \
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[BYTES], stage1[BYTES], stage2[STAGES<DMA, DEEP> == 3 ? BYTES : 16]; \
+    lds8* const s1 = (lds8*)&stage1[0];                                                                    \
     lds8* const s2 = (lds8*)&stage2[0];
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DEEP>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_forward(const GemmArgs A) {
-    PSFM_STAGES(VEC)
+    PSFM_STAGES(VEC, false)
     product<T, BI, BJ, WI, WJ, false, false, VEC, true, false, DEEP>(A, blockIdx.x, gridDim.x, stage0, s1, s2);
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool VEC, bool DZ, bool DEEP>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_pair(const PairArgs A) {
-    PSFM_STAGES(VEC && !DZ)
+    PSFM_STAGES(VEC && !DZ, DZ)
     if (blockIdx.x < A.ndw)
         product<T, BI, BJ, WI, WJ, true, true, VEC, false, DZ, DEEP>(A.dw, blockIdx.x, A.ndw, stage0, s1, s2);
     else

@@ -282,6 +282,22 @@ def test_values_that_are_not_finite(dev, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+def test_an_infinite_gradient_gives_infinities(dev, dtype):
+    """Of the weights' signs, in its row of dx alone; small layers and one whose dz is a pass of its own."""
+    for M, N, K in ((20, 16, 24), (130, 72, 200), (3000, 264, 1200)):
+        t = make(M, N, K, dtype, dev, 5, True)
+        dy = t["dy"].clone()
+        dy[7, 3] = float("inf")
+        for act in (LI.ACT_NONE, LI.ACT_SIGMOID):
+            y = linear_act(t["x"], t["w"], t["bias"], act)
+            dx, db = torch.autograd.grad(y, [t["x"], t["bias"]], dy)
+            assert torch.equal(dx[7], t["w"][3].detach().sign() * float("inf"))
+            assert bool(dx[8:].isfinite().all()) and bool(dx[:7].isfinite().all())
+            assert float(db[3]) == float("inf") and int(db.isfinite().sum()) == N - 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_everything_dropped(dev, dtype):
     t = make(40, 24, 16, dtype, dev, 1, True, True)
     drop, _ = drop_and_keep(40, 24, 1.0, dev)
