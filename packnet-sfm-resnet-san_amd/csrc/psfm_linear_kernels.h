@@ -1,8 +1,8 @@
 // psfm_linear_kernels.h — the pointwise product's kernels, one instance set per type (gfx950).
 //
 //   product   one output tile [BI, BJ] per workgroup on the matrix cores (k_forward: with the epilogue; k_pair:
-//             dx's and dw's tiles in one launch).  LDS holds two stages of 128 bytes of reduction per output row
-//             and column (64 values of 16 bits, 32 of 32): while one is multiplied the next one's global
+//             dx's and dw's tiles in one launch).  LDS holds two or three stages of 128 bytes of reduction per output
+//             row and column (64 values of 16 bits, 32 of 32): while one is multiplied the next ones' global
 //             loads are in flight.  The product is taken as D = Q P^T, so that a lane's four results are
 //             four consecutive columns of one output row.
 //   k_skinny  at most 32 rows: no tiles, W straight from memory into the matrix instructions.
@@ -36,8 +36,7 @@ __device__ __forceinline__ float sigmoidf(float z) { return __builtin_amdgcn_rcp
 
 // The normal distribution function and exp(-z^2 / 2).  fp32: erff.  16 bits: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2),
 // t = 1 / (1 + p x), x >= 0 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: 1.5e-7 of error), which
-// shares its exponential with the density and keeps the lower tail's own scale; erff's two branches took
-// a third of the epilogue.
+// shares its exponential with the density and keeps the lower tail's own scale.
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     e = __expf(-0.5f * z * z);
@@ -101,10 +100,10 @@ __device__ __forceinline__ void times_slope(int act, const float (&z)[N], float 
 #undef PSFM_EACH
 }
 
-// What z is kept in for the backward pass.  The slope is taken at it, so its rounding adds to dz's own: in bf16 that
-// made the gradients of sigmoid 1.7 times as far from 64 bits as one rounding.  fp16 has 8 times
-// bf16's steps in the same bytes; beyond its range (+-65504) every slope has reached its limit.  fp16
-// products keep z in fp32.  ReLU needs the sign alone, in the type itself.
+// What z is kept in for the backward pass.  The slope is taken at it, so its rounding adds to dz's own: |z act''| reaches
+// |act'| (sigmoid, elu), and bf16's would weigh as much as dz's.  fp16 has 8 times bf16's steps in the same
+// bytes; beyond its range (+-65504) every slope has reached its limit.  fp16 products keep z in fp32.  ReLU
+// needs the sign alone, in the type itself.
 template <typename T>
 struct KeptZ {
     using type = float;
@@ -173,9 +172,31 @@ __device__ __forceinline__ void load_run(const T* p, float (&v)[N], int n) {
 }
 
 // ---- the epilogue of columns j .. j + N - 1 (j % 4 = 0; those below J exist) of row i -----------------
+// Its inputs: bias[j ..], or zeros, and res[i, j ..].
+template <typename T, bool FULL, int N>
+__device__ __forceinline__ void bias_run(const LinearEpi& e, int64_t J, int64_t j, float (&b)[N]) {
+    if (FULL && e.bias && j < J) {
+        load_run((const T*)e.bias + j, b, J - j < N ? (int)(J - j) : N);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) b[k] = 0.0f;
+    }
+}
+template <typename T, bool FULL, int N>
+__device__ __forceinline__ void res_run(const LinearEpi& e, int64_t I, int64_t J, int64_t i, int64_t j, T (&r)[N]) {
+    if (!FULL || !e.res || i >= I || j >= J) return;
+    const T* p = (const T*)e.res + i * e.ldr + j;
+    if (J - j >= N) {
+        __builtin_memcpy(r, p, sizeof(T) * N);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < J - j) r[k] = p[k];
+    }
+}
 template <typename T, bool FULL, int N>
 __device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& key, KeepBits<N>& keep, int64_t J, int64_t i,
-                                         int64_t j, float (&v)[N]) {
+                                         int64_t j, float (&v)[N], const float (&b)[N], const T (&r)[N]) {
     const int n = J - j < N ? (int)(J - j) : N;
     const int64_t at = i * J + j;
     if (!FULL) {
@@ -184,12 +205,8 @@ __device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& ke
         store_run((T*)e.out + at, v, n);
         return;
     }
-    if (e.bias) {
-        float b[N];
-        load_run((const T*)e.bias + j, b, n);
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += b[k];
-    }
+    for (int k = 0; k < N; ++k) v[k] += b[k];
     if (e.z) {
         using Z = typename KeptZ<T>::type;
         if (e.act == PSFM_ACT_RELU) {
@@ -206,12 +223,19 @@ __device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& ke
     act_of<T>(e.act, v);
     if (e.drop.rng) drop_run(e.drop, key, keep, J, mask_row(e.drop, i), j, e.drop.scale, v);
     if (e.res) {
-        float r[N];
-        load_run((const T*)e.res + i * e.ldr + j, r, n);
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += r[k];
+        for (int k = 0; k < N; ++k) v[k] += (float)r[k];
     }
     store_run((T*)e.out + at, v, n);
+}
+template <typename T, bool FULL, int N>
+__device__ __forceinline__ void epilogue(const LinearEpi& e, const PhiloxKey& key, KeepBits<N>& keep, int64_t I, int64_t J,
+                                         int64_t i, int64_t j, float (&v)[N]) {
+    float b[N];
+    T r[N];
+    bias_run<T, FULL>(e, J, j, b);
+    res_run<T, FULL>(e, I, J, i, j, r);
+    epilogue<T, FULL>(e, key, keep, J, i, j, v, b, r);
 }
 
 // ---- LDS images ----------------------------------------------------------------------------
@@ -515,7 +539,7 @@ template <typename T>
 __device__ __forceinline__ f4 mma(u4v a, u4v b, f4 c) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)   // the four 16-value steps take the same reduction order of both operands
+        for (int i = 0; i < 4; ++i)   // the four steps of four values take the same reduction order of both operands
             c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
         return c;
     } else if constexpr (__is_same(T, __bf16)) {
@@ -783,7 +807,7 @@ __device__ __forceinline__ void product(const GemmArgs& A, uint32_t id, uint32_t
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[4 * q + k] = x[k];
                 }
-                epilogue<T, FULL>(A.e, key, keep, A.J, ib + i, j0 + col, v);
+                epilogue<T, FULL>(A.e, key, keep, A.I, A.J, ib + i, j0 + col, v);
             }
         }
     }
@@ -826,6 +850,13 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
     f4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = f4{0, 0, 0, 0};
+    // the epilogue's thread, in the first MT waves: 4 columns (lane group g of the results) of one row.  Its inputs
+    // are on their way while W is read (1 x 512 x 512 bf16: 4.25 -> 4.08 us; in the tiles the registers cost more than that gave).
+    const int64_t i = wave * 16 + n, jj = j0 + 4 * g;
+    float bias[4];
+    T res[4];
+    bias_run<T, true>(A.e, A.N, jj, bias);
+    res_run<T, true>(A.e, A.M, A.N, i, jj, res);
     for (int64_t k0 = (int64_t)wave * 2 * STEP; k0 < A.K; k0 += SKINNY_WAVES * U * STEP) {
         u4v fw[U], fx[U][MT];
 #pragma unroll
@@ -835,8 +866,8 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
             fw[u] = load_n<T, VEC>(w + (have ? k : 0), j < A.N ? have : 0);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const int64_t i = m * 16 + n;
-                fx[u][m] = load_n<T, VEC>((const T*)A.x + (i < A.M && have ? i * A.ldx + k : 0), i < A.M ? have : 0);
+                const int64_t row = m * 16 + n;
+                fx[u][m] = load_n<T, VEC>((const T*)A.x + (row < A.M && have ? row * A.ldx + k : 0), row < A.M ? have : 0);
             }
         }
 #pragma unroll
@@ -847,11 +878,9 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
 #pragma unroll
     for (int m = 0; m < MT; ++m) part[wave][m][l] = acc[m];
     __syncthreads();
-    // 4 columns (lane group g of the results) of one row a thread
+    if (wave >= MT) return;
     PhiloxKey key{};
     if (A.e.drop.rng) key = philox_key(A.e.drop.rng);
-    if (wave >= MT) return;
-    const int64_t i = wave * 16 + n, jj = j0 + 4 * g;
     if (i >= A.M || jj >= A.N) return;
     float v[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -859,7 +888,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] += part[s][wave][l][k];
     KeepBits<4> keep;
-    epilogue<T, true>(A.e, key, keep, A.N, i, jj, v);
+    epilogue<T, true>(A.e, key, keep, A.N, i, jj, v, bias, res);
 }
 
 // Split products: 256 / SL groups of four columns a workgroup, SL threads a group, each summing every SL-th split;
@@ -896,7 +925,7 @@ __device__ __forceinline__ void join(const GemmArgs& A, uint32_t block, f4* sums
     PhiloxKey key{};
     if (FULL && A.e.drop.rng) key = philox_key(A.e.drop.rng);
     KeepBits<4> keep;
-    epilogue<T, FULL>(A.e, key, keep, A.J, i, j, v);
+    epilogue<T, FULL>(A.e, key, keep, A.I, A.J, i, j, v);
 }
 
 constexpr int JOIN_FEW = 8, JOIN_LANES = 16;   // up to JOIN_FEW splits one thread a group sums them all
