@@ -99,7 +99,8 @@ struct Tile {
 constexpr Tile LINEAR_TILES[] = {{64, 64}, {128, 128}, {256, 256}};
 constexpr int LINEAR_NTILES = 3;   // 32-bit types: the first two
 constexpr int DZ_THREADS = 256;
-// chunks of columns in a k_dz workgroup: all of a narrow layer's, 32 of a wide one's
+// Chunks of columns in a k_dz workgroup: all of a narrow layer's, 32 of a wide one's (184320 x 64 bf16: 15.1 us with 8, 32.8
+// with 32; 100000 x 8: 11.0, 20.0; 4096 x 24: 6.1, 6.3).
 constexpr int DZ_NARROW = 8, DZ_WIDE = 32;
 constexpr int SKINNY_ROWS = 32;    // at most
 

@@ -55,6 +55,7 @@ struct Plan {
     int variant;
     int64_t ti, tj, rsplit;
     int splits;
+    double alone, busy, join;   // estimates: the larger of the first two, and the join
     int64_t blocks() const { return ti * tj * splits; }
 };
 
@@ -64,30 +65,40 @@ struct Plan {
 // splits over products from 300 x 500 x 1200 to 16384 x 1024 x 256 (I x J x R); the choice was within a seventh of the best
 // one (bf16 1024 x 1024 x 1024: 8.0 us as chosen, 64 tiles in one piece; two pieces 13.8; 128 tiles 16.7; 256 tiles 33.
 // 256 x 1024 x 4096: 11.1 in four pieces, 12.2 in two.  512 x 4096 x 4096: 26.9, 128 tiles in four pieces 31.3).  Rows that
-// are no whole chunks go through registers, and wait for memory half as long again.
+// are no whole chunks go through registers, and wait for memory half as long again.  STAGED: dz made on the way, whose
+// every stage waits for its loads and the activation's slope (8192 x 2048, reduction 128 in bf16: 41 us in 16 pieces, 42 in
+// 8, 220 in one).
 struct TileTime {
     double alone, busy;
 };
-constexpr TileTime TIMES16[] = {{0.42, 0.22}, {1.15, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}};
+constexpr TileTime TIMES16[] = {{0.42, 0.22}, {1.15, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}},
+                   STAGED16[] = {{1.75, 1.15}}, STAGED32[] = {{1.45, 1.0}};
 
-Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1) {
+bool chunks(const psfm_linear* d) {
+    const int64_t v = 16 / size_of(d->dtype);
+    return d->N % v == 0 && d->K % v == 0 && d->ldx % v == 0;
+}
+
+Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1, bool staged = false) {
     static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512};
     const bool wide = d->dtype == PSFM_DTYPE_F32;
-    const TileTime* times = wide ? TIMES32 : TIMES16;
-    const int64_t stage = 128 / size_of(d->dtype), stages = up(R, stage), v16 = 16 / size_of(d->dtype);
-    const double wait = d->N % v16 || d->K % v16 || d->ldx % v16 ? 1.5 : 1.0;
-    Plan best{0, 0, 0, 0, 1};
+    const TileTime* times = staged ? (wide ? STAGED32 : STAGED16) : wide ? TIMES32 : TIMES16;
+    const int64_t stage = 128 / size_of(d->dtype), stages = up(R, stage);
+    const double wait = chunks(d) ? 1.0 : 1.5;
+    Plan best{0, 0, 0, 0, 1, 0, 0, 0};
     double least = 0;
-    for (int v = std::min(largest, wide ? 1 : 2); v >= 0; --v) {
+    for (int v = staged ? 0 : std::min(largest, wide ? 1 : 2); v >= 0; --v) {
         const int64_t ti = up(I, LINEAR_TILES[v].bi), tj = up(J, LINEAR_TILES[v].bj);
         for (const int want : SPLITS) {
             const int64_t per = std::max<int64_t>(1, up(stages, want)), n = std::max<int64_t>(1, up(stages, per));
             if (want > 1 && (per < 2 || ti * tj * n > 4096)) break;
-            const double blocks = (double)ti * (double)tj * (double)n, load = std::min(1.0, blocks / 512);
-            double t = (double)per * std::max(times[v].alone * wait * (0.64 + 0.36 * load),
-                                              times[v].busy * (double)up((int64_t)std::min(blocks, 1e15), 256));
-            if (n > 1) t += 4.0 + 0.15 * (double)std::min<int64_t>(n, 8) + 0.012 * (double)n + (double)n * (double)I * (double)J * 8 / 5e6;
-            if (best.rsplit == 0 || t < least) least = t, best = Plan{v, ti, tj, per * stage, (int)n};
+            const double blocks = (double)ti * (double)tj * (double)n, load = staged ? 1.0 : std::min(1.0, blocks / 512);
+            const double alone = (double)per * times[v].alone * wait * (0.64 + 0.36 * load);
+            const double busy = (double)per * times[v].busy * (double)up((int64_t)std::min(blocks, 1e15), 256);
+            const double join = n == 1 ? 0.0 : 4.0 + 0.15 * (double)std::min<int64_t>(n, 8) + 0.012 * (double)n +
+                                                   (double)n * (double)I * (double)J * 8 / 5e6;
+            const double t = std::max(alone, busy) + join;
+            if (best.rsplit == 0 || t < least) least = t, best = Plan{v, ti, tj, per * stage, (int)n, alone, busy, join};
         }
     }
     return best;
@@ -99,7 +110,10 @@ bool mult(const void* p, int64_t ld, int64_t edge, int64_t v) {
     return ((uintptr_t)p & 15) == 0 && ld % v == 0 && edge % v == 0;
 }
 
-bool skinny(const psfm_linear* d) { return d->M <= SKINNY_ROWS; }
+// Rows that one matrix instruction takes, or two where W's rows are short.  4096 x 4096 bf16, 16 rows: 9.9 us, 10.2 in
+// tiles; 32 rows: 13.6, 11.2.  1024 x 1024, 32 rows: 5.1, 6.5.  fp32 4096 x 4096, 16 rows: 20.1, 27.0; 32 rows: 28.9,
+// 27.8; 512 x 512, 32 rows: 6.2, 7.9.
+bool skinny(const psfm_linear* d) { return d->M <= 16 || (d->M <= SKINNY_ROWS && d->K * size_of(d->dtype) < 4096); }
 
 struct DzPlan {
     int64_t gx, gy, rows;
@@ -126,23 +140,42 @@ struct BwdPlan {
     DzPlan cols;
 };
 
-// The products share a launch where they share a tile.  They make dz themselves where that repeats little: every tile
-// column of either makes it once, in the smallest tiles, and a pass of its own costs a launch and dz's way to
-// memory and back.
+// The time of the products together: they share a launch where they share a tile.
+double together(const BwdPlan& b) {
+    const Plan none{}, &x = b.dx ? b.pdx : none, &w = b.dw ? b.pdw : none;
+    if (x.variant != w.variant) return std::max(x.alone, x.busy) + std::max(w.alone, w.busy) + std::max(x.join, w.join);
+    return std::max({x.alone, w.alone, x.busy + w.busy}) + std::max(x.join, w.join);
+}
+
+constexpr int64_t FEW_DZ = 1 << 15;
+
+// The products make dz themselves, in the smallest tiles, where that should take less time than a pass of its own, a launch
+// and dz's way to memory and back.  bf16, both gradients and the bias's (rows x K x N): 64 x 4096 x 64 5.2 us,
+// 8.3 with a pass; 480 x 64 x 64 9.5, 10.9; 480 x 512 x 256 13.8, 11.9; 184320 x 128 x 64 64, 51; 8192 x 256 x 2048 126, 52.
+// fp32: 480 x 64 x 256 10.2, 15.8; 30720 x 128 x 64 29, 35; 184320 x 256 x 64 195, 177; 8192 x 256 x 2048 242, 186.  A pass
+// rounds dz to the type once more, 16 bits off by up to sqrt(2) of one rounding where that averages over many values; with
+// few of them (1.49 was seen at 1500) the products make it for some microseconds more too.  The choice is the layer's, for all gradients together: what one of them is does not depend
+// on which others are asked for.
 BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db) {
     BwdPlan b{};
     const bool any = d->M > 0 && d->N > 0, make = d->act != PSFM_ACT_NONE || drop_of(d).rng;
+    b.dx = b.dw = any && d->K > 0;
+    // turned operands of odd rows leave the largest tile no registers (8191 x 1023 over 8191, bf16: 636 us, 172 in the next one)
+    const int largest = chunks(d) ? LINEAR_NTILES - 1 : 1;
+    auto plans = [&](bool staged) {
+        if (d->M > 0 && d->K > 0) b.pdx = plan(d, d->M, d->K, d->N, largest, staged);
+        if (d->N > 0 && d->K > 0) b.pdw = plan(d, d->N, d->K, d->M, largest, staged);
+        return together(b);
+    };
+    const double moved = (double)d->M * (double)d->N * size_of(d->dtype) * (2 + (d->act != PSFM_ACT_NONE));
+    const double few = size_of(d->dtype) == 2 && d->M * d->N < FEW_DZ ? 4.0 : 0.0;
+    b.stage = make && b.dx && plans(true) < plans(false) + 5.5 + few + moved / 5e6;
+    plans(b.stage);
     b.dx = want_dx && d->M > 0 && d->K > 0;
     b.dw = want_dw && d->N > 0 && d->K > 0;
-    const int64_t columns = (b.dx + b.dw) * up(d->K, LINEAR_TILES[0].bj);
-    const bool cheap = columns <= 4 || (double)columns * (double)d->M * (double)d->N < 8e6;
-    b.stage = any && (b.dx || b.dw) && cheap && (make || (want_db && b.dw));
-    const int largest = b.stage ? 0 : LINEAR_NTILES - 1;
-    if (b.dx) b.pdx = plan(d, d->M, d->K, d->N, largest);
-    if (b.dw) b.pdw = plan(d, d->N, d->K, d->M, largest);
-    b.pass = any && !b.stage && ((make && (b.dx || b.dw)) || want_db);
-    if (b.stage && want_db && !b.dw) b.pass = true;      // the column sums alone
-    b.dz = b.pass && !b.stage && make && (b.dx || b.dw);
+    b.stage = b.stage && (b.dx || b.dw);
+    b.dz = make && !b.stage && any && (b.dx || b.dw);
+    b.pass = b.dz || (want_db && any && !(b.stage && b.dw));   // the latter: the column sums alone
     b.cols = dz_plan(d->dtype, d->M, d->N);
     b.parts = !want_db || !any ? 0 : b.pass ? b.cols.gy : b.pdw.splits > 1 ? b.pdw.splits : 0;
     b.cols_at = b.dz ? aligned(d->M * d->N * size_of(d->dtype)) : 0;
@@ -150,6 +183,12 @@ BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db)
     b.dwp_at = b.dxp_at + (b.dx ? aligned(part_bytes(b.pdx, d->M, d->K)) : 0);
     b.bytes = b.dwp_at + (b.dw ? part_bytes(b.pdw, d->N, d->K) : 0);
     return b;
+}
+
+// whole chunks at other addresses: the next tile, whose splits are the same
+void retile(Plan& p, int64_t I, int64_t J) {
+    if (p.variant < 2) return;
+    p.variant = 1, p.ti = up(I, LINEAR_TILES[1].bi), p.tj = up(J, LINEAR_TILES[1].bj);
 }
 
 void set(GemmArgs& a, const Plan& p, void* parts) {
@@ -202,8 +241,14 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
     const bool any = d->M > 0 && d->N > 0;
     if (any && (!dy || (d->act != PSFM_ACT_NONE && !z) || (dx && d->K > 0 && !w) || (dw && d->K > 0 && !x)))
         return fail(-9, "psfm_linear_bwd: null tensor");
-    const BwdPlan b = bwd_plan(d, dx, dw, db);
+    BwdPlan b = bwd_plan(d, dx, dw, db);
     if (b.bytes > 0 && !ws) return fail(-10, "psfm_linear_bwd: no workspace");
+    const void* dz = b.dz ? ws : dy;
+    const int64_t v = 16 / size_of(d->dtype);
+    const bool vec = d->N % v == 0 && d->K % v == 0 && ((uintptr_t)dz & 15) == 0 &&
+                     (!b.stage || d->act == PSFM_ACT_NONE || ((uintptr_t)z & 15) == 0) &&
+                     (!b.dx || ((uintptr_t)w & 15) == 0) && (!b.dw || mult(x, d->ldx, d->K, v));
+    if (!vec) retile(b.pdx, d->M, d->K), retile(b.pdw, d->N, d->K);
     const int64_t most = 0x7fffffff;
     if (b.cols.gx > most || (b.dx && b.pdx.blocks() > most / 2) || (b.dw && b.pdw.blocks() > most / 2))
         return fail(-8, "psfm_linear_bwd: more tiles than a launch holds");
@@ -218,8 +263,6 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
         a.dz.cols = b.parts ? cols : nullptr;
         if (const int rc = status(o.dz(a, b.cols.gx, b.cols.gy, s), "psfm_linear_bwd: dz launch")) return rc;
     }
-    const void* dz = b.dz ? ws : dy;
-    const int64_t v = 16 / size_of(d->dtype);
     PairArgs pair{};
     if (b.dx) {
         GemmArgs& a = pair.dx;
@@ -234,12 +277,10 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
         if (db && !b.pass) (b.parts ? (void*&)a.dz.cols : a.dz.db) = b.parts ? (void*)cols : db;
         set(a, b.pdw, at + b.dwp_at);
     }
-    const bool vec = d->N % v == 0 && d->K % v == 0 && ((uintptr_t)dz & 15) == 0 && (!make.z || ((uintptr_t)z & 15) == 0) &&
-                     (!b.dx || ((uintptr_t)w & 15) == 0) && (!b.dw || mult(x, d->ldx, d->K, v));
-    const bool together = b.dx && b.dw && b.pdx.variant == b.pdw.variant;
-    for (int part = 0; part < (together ? 1 : 2); ++part) {
+    const bool one = b.dx && b.dw && b.pdx.variant == b.pdw.variant;
+    for (int part = 0; part < (one ? 1 : 2); ++part) {
         pair.ndx = b.dx && part == 0 ? pair.dx.blocks() : 0;
-        pair.ndw = b.dw && (together || part == 1) ? pair.dw.blocks() : 0;
+        pair.ndw = b.dw && (one || part == 1) ? pair.dw.blocks() : 0;
         if (pair.ndx + pair.ndw == 0) continue;
         const int rc = o.pair(pair.ndx ? b.pdx.variant : b.pdw.variant, vec, b.stage, pair, s);
         if (rc) return status(rc, "psfm_linear_bwd: launch");
@@ -247,7 +288,7 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
     FinishArgs f{};
     f.dx = pair.dx, f.dw = pair.dw;
     // no rows or no products to sum: the bias gradient of no parts is zero
-    if (db && d->N > 0 && (b.parts || !any || !b.stage || !b.dw)) f.cols = cols, f.parts = b.parts, f.N = d->N, f.alpha = drop.scale, f.db = db;
+    if (db && d->N > 0 && (b.parts || !any)) f.cols = cols, f.parts = b.parts, f.N = d->N, f.alpha = drop.scale, f.db = db;
     return status(o.finish(f, s), "psfm_linear_bwd: finish launch");
 }
 

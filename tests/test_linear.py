@@ -224,6 +224,23 @@ def test_layouts_and_alignment(dev, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+def test_large_products_at_odd_addresses(dev, dtype):
+    """Whole chunks of rows from bases that are no multiple of 16 bytes, at a size whose gradients take the largest
+    tiles; and the same from odd rows."""
+    for M, N, K in ((4096, 8192, 2048), (2050, 4097, 1023)):
+        t = make(M, N, K, dtype, dev, 9, False, grad=False)
+        buf = torch.empty(M * K + 1, device=dev, dtype=dtype)
+        x = buf[1:].view(M, K).copy_(t["x"]).requires_grad_(True)
+        w = t["w"].requires_grad_(True)
+        y = linear_act(x, w, None, LI.ACT_SILU)
+        ref = formulas(x, w, None, None, "silu", None, 0, t["dy"])
+        check(y, ref["y"], "y")
+        for k, got in zip(("dx", "dw"), torch.autograd.grad(y, [x, w], t["dy"])):
+            check(got, ref[k], k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_images(dev, dtype):
     """conv1x1_act on NCHW and channels_last images against F.conv2d's formula."""
     g = torch.Generator().manual_seed(2)
