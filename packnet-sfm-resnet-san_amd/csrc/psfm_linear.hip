@@ -61,7 +61,9 @@ struct Plan {
 
 // The tile and the splits of the reduction that should take least time, from what a stage of 128 bytes of reduction
 // takes (us): `alone` where a CU has one or two workgroups and waits for memory, `busy` per workgroup where it
-// has enough of them; splits add a launch and their way through memory.  From a sweep of every tile and 1 .. 16
+// has enough of them, and from `out`, a tile's way through the forward epilogue (short reductions live from small tiles: 50000 x
+// 256 over 64 in bf16 14.3, 17.9 and 18.5 us in tiles of 64, 128 and 256; over 1024 44.4, 41.9, 41.0); splits write no
+// tile but add a launch and their way through memory.  From a sweep of every tile and 1 .. 16
 // splits over products from 300 x 500 x 1200 to 16384 x 1024 x 256 (I x J x R); the choice was within a seventh of the best
 // one (bf16 1024 x 1024 x 1024: 8.0 us as chosen, 64 tiles in one piece; two pieces 13.8; 128 tiles 16.7; 256 tiles 33.
 // 256 x 1024 x 4096: 11.1 in four pieces, 12.2 in two.  512 x 4096 x 4096: 26.9, 128 tiles in four pieces 31.3).  Rows that
@@ -69,17 +71,19 @@ struct Plan {
 // every stage waits for its loads and the activation's slope (8192 x 2048, reduction 128 in bf16: 41 us in 16 pieces, 42 in
 // 8, 220 in one).
 struct TileTime {
-    double alone, busy;
+    double alone, busy, out;
 };
-constexpr TileTime TIMES16[] = {{0.42, 0.22}, {1.15, 0.5}, {2.0, 2.0}}, TIMES32[] = {{0.8, 0.61}, {2.4, 2.39}},
-                   STAGED16[] = {{1.75, 1.15}}, STAGED32[] = {{1.45, 1.0}};
+constexpr TileTime TIMES16[] = {{0.42, 0.22, 0.4}, {1.15, 0.5, 3.4}, {2.0, 2.0, 13.0}},
+                   TIMES32[] = {{0.8, 0.61, 0.5}, {2.4, 2.39, 3.0}}, STAGED16[] = {{1.75, 1.15, 0}},
+                   STAGED32[] = {{1.45, 1.0, 0}};
 
 bool chunks(const psfm_linear* d) {
     const int64_t v = 16 / size_of(d->dtype);
     return d->N % v == 0 && d->K % v == 0 && d->ldx % v == 0;
 }
 
-Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = LINEAR_NTILES - 1, bool staged = false) {
+Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, bool forward, int largest = LINEAR_NTILES - 1,
+          bool staged = false) {
     static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512};
     const bool wide = d->dtype == PSFM_DTYPE_F32;
     const TileTime* times = staged ? (wide ? STAGED32 : STAGED16) : wide ? TIMES32 : TIMES16;
@@ -93,8 +97,9 @@ Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, int largest = L
             const int64_t per = std::max<int64_t>(1, up(stages, want)), n = std::max<int64_t>(1, up(stages, per));
             if (want > 1 && (per < 2 || ti * tj * n > 4096)) break;
             const double blocks = (double)ti * (double)tj * (double)n, load = staged ? 1.0 : std::min(1.0, blocks / 512);
-            const double alone = (double)per * times[v].alone * wait * (0.64 + 0.36 * load);
-            const double busy = (double)per * times[v].busy * (double)up((int64_t)std::min(blocks, 1e15), 256);
+            const double rounds = (double)up((int64_t)std::min(blocks, 1e15), 256), out = forward && n == 1 ? times[v].out : 0.0;
+            const double alone = (double)per * times[v].alone * wait * (0.64 + 0.36 * load) + out;
+            const double busy = ((double)per * times[v].busy + out) * rounds;
             const double join = n == 1 ? 0.0 : 4.0 + 0.15 * (double)std::min<int64_t>(n, 8) + 0.012 * (double)n +
                                                    (double)n * (double)I * (double)J * 8 / 5e6;
             const double t = std::max(alone, busy) + join;
@@ -163,8 +168,8 @@ BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db)
     // turned operands of odd rows leave the largest tile no registers (8191 x 1023 over 8191, bf16: 636 us, 172 in the next one)
     const int largest = chunks(d) ? LINEAR_NTILES - 1 : 1;
     auto plans = [&](bool staged) {
-        if (d->M > 0 && d->K > 0) b.pdx = plan(d, d->M, d->K, d->N, largest, staged);
-        if (d->N > 0 && d->K > 0) b.pdw = plan(d, d->N, d->K, d->M, largest, staged);
+        if (d->M > 0 && d->K > 0) b.pdx = plan(d, d->M, d->K, d->N, false, largest, staged);
+        if (d->N > 0 && d->K > 0) b.pdw = plan(d, d->N, d->K, d->M, false, largest, staged);
         return together(b);
     };
     const double moved = (double)d->M * (double)d->N * size_of(d->dtype) * (2 + (d->act != PSFM_ACT_NONE));
@@ -201,7 +206,7 @@ extern "C" {
 
 int64_t psfm_linear_fwd_ws_bytes(const psfm_linear* d) {
     if (check(d)) return -1;
-    return skinny(d) ? 0 : part_bytes(plan(d, d->M, d->N, d->K), d->M, d->N);
+    return skinny(d) ? 0 : part_bytes(plan(d, d->M, d->N, d->K, true), d->M, d->N);
 }
 
 int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const void* bias, const void* res, void* y,
@@ -219,7 +224,7 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
         if (up(d->N, 16) > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more columns than a launch holds");
         return status(o.skinny(vec, SkinnyArgs{x, w, d->ldx, d->M, d->N, d->K, e}, s), "psfm_linear_fwd: launch");
     }
-    const Plan p = plan(d, d->M, d->N, d->K);
+    const Plan p = plan(d, d->M, d->N, d->K, true);
     if (p.splits > 1 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
     if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more tiles than a launch holds");
     GemmArgs a{};
