@@ -172,6 +172,11 @@ at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
 
 bool wants(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Forward-mode derivatives are refused: the result would silently carry none.
+void refuse_tangents(const at::Tensor& t, const char* what) {
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), what, " has no forward-mode derivative");
+}
+
 // A gradient asked for with a graph of its own (create_graph) raises when that is differentiated.
 at::Tensor once(const at::Tensor& g, const char* what) {
     if (!g.defined() || !at::GradMode::is_enabled()) return g;
@@ -245,6 +250,7 @@ at::Tensor linear_act(const at::Tensor& x_, const at::Tensor& weight_, const std
     refuse_foreign_capture();
     const at::Tensor bias_in = bias_.value_or(at::Tensor()), res_in = residual_.value_or(at::Tensor()),
                      rng = rng_.value_or(at::Tensor());
+    for (const at::Tensor* t : {&x_, &weight_, &bias_in, &res_in}) refuse_tangents(*t, "linear_act");
     const bool grad_x = wants(x_), grad_w = wants(weight_), grad_b = wants(bias_in);
     std::shared_ptr<LinearActBackward> node;
     const bool in_capture = capturing();
@@ -339,6 +345,7 @@ at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residua
                    bool channels) {
     refuse_foreign_capture();
     const at::Tensor res = residual.value_or(at::Tensor());
+    for (const at::Tensor* t : {&x, &res}) refuse_tangents(*t, "dropout");
     const int64_t share = mask_rows(x.sizes(), channels);
     std::shared_ptr<DropoutBackward> node;
     if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {

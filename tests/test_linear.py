@@ -448,6 +448,43 @@ def test_second_derivatives_are_refused(dev):
 
 
 @gpu
+def test_forward_mode_derivatives_are_refused(dev):
+    import torch.autograd.forward_ad as fwd
+    t = make(4, 8, 6, torch.float32, dev, 3, True, True, grad=False)
+    drop = Drop(0.5, pair(1, 2, dev))
+    with fwd.dual_level():
+        for k in ("x", "w", "bias", "res"):
+            a = {**t, k: fwd.make_dual(t[k], torch.ones_like(t[k]))}
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                linear_act(a["x"], a["w"], a["bias"], LI.ACT_SILU, a["res"])
+        dual = fwd.make_dual(t["res"], torch.ones_like(t["res"]))
+        for args in ((dual, drop), (t["res"], drop, dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                dropout(*args)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_checkpointed_and_offloaded(dev, dtype):
+    """A forward that is run again for its backward makes the same mask; saved tensors may rest on the host."""
+    from torch.utils.checkpoint import checkpoint
+    t = make(300, 72, 136, dtype, dev, 8, True, True)
+    leaves = [t[k] for k in ("x", "w", "bias", "res")]
+    drop = Drop(0.4, pair(6, 7, dev))
+
+    def block(x, w, b, r):
+        return dropout(linear_act(x, w, b, LI.ACT_RELU, r, drop), drop, r)
+
+    want = torch.autograd.grad(block(*leaves), leaves, t["dy"])
+    again = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, t["dy"])
+    with torch.autograd.graph.save_on_cpu():
+        y = block(*leaves)
+    away = torch.autograd.grad(y, leaves, t["dy"])
+    for w, a, b in zip(want, again, away):
+        assert torch.equal(w, a) and torch.equal(w, b)
+
+
+@gpu
 def test_saved_tensors_changed_in_place_are_refused(dev):
     for change, act in (("x", LI.ACT_NONE), ("w", LI.ACT_NONE), ("y", LI.ACT_RELU)):
         t = make(40, 24, 16, torch.bfloat16, dev, 1, False)
