@@ -184,13 +184,33 @@ at::Tensor once(const at::Tensor& g, const char* what) {
     return torch::autograd::DelayedError(std::string(what) + " cannot be differentiated twice", 1).apply(std::move(v))[0];
 }
 
+// A saved tensor as it was kept, if it was.  Saved-tensor hooks may give back another one: it need not have the strides
+// of the one that they took (a slice of a wider buffer comes back dense from the host), but its shape, type and
+// device.
+at::Tensor unpacked(const SavedVariable& v, const std::shared_ptr<torch::autograd::Node>& node, at::IntArrayRef shape,
+                    at::ScalarType type, c10::Device device, const char* what) {
+    const at::Tensor t = v.unpack(node);
+    TORCH_CHECK(!t.defined() || (t.sizes() == shape && t.scalar_type() == type && t.device() == device), what,
+                ": saved as ", shape, " ", type, " on ", device, ", given back as ", t.sizes(), " ", t.scalar_type(), " on ",
+                t.device());
+    return t;
+}
+
+at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
 // ---- linear_act ------------------------------------------------------------------------------------
 struct LinearMeta {
-    at::DimVector xshape;
-    int64_t ldx, N, K, share;
+    at::DimVector xshape, rshape;
+    int64_t N, K, share;
     int32_t act;
     double p;
 };
+
+// what z is kept in: psfm_linear_fwd
+at::ScalarType kept_type(at::ScalarType x, int act) {
+    if (act == PSFM_ACT_RELU) return x;
+    return x == at::kBFloat16 ? at::kHalf : at::kFloat;
+}
 
 struct LinearActBackward : public torch::autograd::Node {
     SavedVariable x, weight, z, rng;
@@ -216,14 +236,23 @@ struct LinearActBackward : public torch::autograd::Node {
                    db = task_should_compute_output(2);
         if (dx || dw || db) {
             at::AutoDispatchBelowADInplaceOrView below;
-            const at::Tensor xs = x.unpack(shared_from_this()), ws = weight.unpack(shared_from_this()),
-                             zs = z.unpack(shared_from_this()), rs = rng.unpack(shared_from_this());
             const at::Tensor g = dy.contiguous();
-            c10::DeviceGuard guard(g.device());
+            const at::ScalarType type = g.scalar_type();
+            const c10::Device device = g.device();
+            const auto self = shared_from_this();
+            c10::DeviceGuard guard(device);
+            int64_t ldx = m.K;
+            at::DimVector zshape = m.xshape;
+            zshape.back() = m.N;
+            at::Tensor xs = unpacked(x, self, m.xshape, type, device, "linear_act: x");
+            if (xs.defined()) xs = as_rows(xs, ldx);
+            const at::Tensor ws = dense(unpacked(weight, self, {m.N, m.K}, type, device, "linear_act: weight")),
+                             zs = dense(unpacked(z, self, zshape, kept_type(type, m.act), device, "linear_act: z")),
+                             rs = dense(unpacked(rng, self, m.rshape, at::kLong, device, "linear_act: rng"));
             if (dx) out[0] = at::empty(m.xshape, g.options());
             if (dw) out[1] = at::empty({m.N, m.K}, g.options());
             if (db) out[2] = at::empty({m.N}, g.options());
-            const psfm_linear d{lead_of(m.xshape), m.N, m.K, m.ldx, 0, dtype_of(g), m.act, m.p, m.share,
+            const psfm_linear d{lead_of(m.xshape), m.N, m.K, ldx, 0, dtype_of(g), m.act, m.p, m.share,
                                 (const int64_t*)at_of(rs)};
             const int64_t n = entry.bwd_ws(&d, dx, dw, db);
             TORCH_CHECK(n >= 0, "psfm_linear_bwd_ws_bytes failed: ", entry.linear_error());
@@ -237,12 +266,6 @@ struct LinearActBackward : public torch::autograd::Node {
         return out;
     }
 };
-
-// what z is kept in: psfm_linear_fwd
-at::ScalarType kept_type(const at::Tensor& x, int act) {
-    if (act == PSFM_ACT_RELU) return x.scalar_type();
-    return x.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat;
-}
 
 at::Tensor linear_act(const at::Tensor& x_, const at::Tensor& weight_, const std::optional<at::Tensor>& bias_, int64_t act,
                       const std::optional<at::Tensor>& residual_, double p, const std::optional<at::Tensor>& rng_,
@@ -267,20 +290,21 @@ at::Tensor linear_act(const at::Tensor& x_, const at::Tensor& weight_, const std
     {
         at::AutoDispatchBelowADInplaceOrView below;
         c10::DeviceGuard guard(x_.device());
-        int64_t ldr = 0;
-        x = as_rows(x_, m.ldx);
+        int64_t ldx = 0, ldr = 0;
+        x = as_rows(x_, ldx);
         weight = weight_.contiguous();
         const at::Tensor bias = bias_in.defined() ? bias_in.contiguous() : bias_in,
                          res = res_in.defined() ? as_rows(res_in, ldr) : res_in;
         m.xshape = at::DimVector(x.sizes());
         m.N = weight.size(0), m.K = weight.size(1), m.act = (int32_t)act, m.p = p;
         m.share = mask_rows(m.xshape, channels);
+        if (rng.defined()) m.rshape = at::DimVector(rng.sizes());
         at::DimVector shape = m.xshape;
         shape.back() = m.N;
         y = at::empty(shape, x.options());
         if (node && act != PSFM_ACT_NONE && !from_y && (grad_x || grad_w || grad_b))
-            z = at::empty(shape, x.options().dtype(kept_type(x, (int)act)));
-        const psfm_linear d{lead_of(m.xshape), m.N, m.K, m.ldx, ldr, dtype_of(x), m.act, p, m.share,
+            z = at::empty(shape, x.options().dtype(kept_type(x.scalar_type(), (int)act)));
+        const psfm_linear d{lead_of(m.xshape), m.N, m.K, ldx, ldr, dtype_of(x), m.act, p, m.share,
                             (const int64_t*)at_of(rng)};
         const int64_t n = entry.fwd_ws(&d);
         TORCH_CHECK(n >= 0, "psfm_linear_fwd_ws_bytes failed: ", entry.linear_error());
@@ -320,6 +344,7 @@ at::Tensor drop_launch(const at::Tensor& x_, const at::Tensor& res_, double p, c
 
 struct DropoutBackward : public torch::autograd::Node {
     SavedVariable rng;
+    at::DimVector rshape;
     double p = 0;
     int64_t share = 1;
     Live live;
@@ -334,7 +359,7 @@ struct DropoutBackward : public torch::autograd::Node {
         variable_list out(2);
         const at::Tensor& dy = grads[0];
         if (!dy.defined()) return out;
-        const at::Tensor r = rng.unpack(shared_from_this());
+        const at::Tensor r = dense(unpacked(rng, shared_from_this(), rshape, at::kLong, dy.device(), "dropout: rng"));
         if (task_should_compute_output(0)) out[0] = once(drop_launch(dy, at::Tensor(), p, r, share), "dropout");
         if (task_should_compute_output(1)) out[1] = dy;
         return out;
@@ -360,6 +385,7 @@ at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residua
     at::Tensor y = drop_launch(x, res, p, rng, share);
     if (node) {
         node->p = p, node->share = share;
+        node->rshape = at::DimVector(rng.sizes());
         node->rng = SavedVariable(rng, false);
         torch::autograd::set_history(y, node);
     }

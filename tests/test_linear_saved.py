@@ -1,0 +1,79 @@
+"""What linear_act and dropout keep for their backward pass, given back by saved-tensor hooks: from the host, with other
+strides, as another tensor.  Gradients against the formulas in float64 (test_linear.formulas derives the tolerances)."""
+import pytest
+import torch
+
+import packnet_sfm_amd  # noqa: F401
+from packnet_sfm_amd.networks.layers import linear as LI
+from packnet_sfm_amd.networks.layers.dropout import Drop, dropout
+from packnet_sfm_amd.networks.layers.linear import linear_act
+from test_dropout import pair
+from test_linear import ACTS, TYPES, check, drop_and_keep, formulas, make
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a ROCm GPU")
+    return torch.device("cuda", 0)
+
+
+def restrided(t):
+    """t's values at strides that no operator makes: turned, or every third value."""
+    if t.dim() >= 2:
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    return torch.stack((t, t, t), -1)[..., 1]
+
+
+HOOKS = {"host": (lambda t: t.cpu(), lambda t: t.cuda()), "turned": (restrided, lambda t: t),
+         "wider": (lambda t: torch.cat((t, t), -1)[..., :t.shape[-1]] if t.dim() else t, lambda t: t)}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K,pad", [(6, 16, 8, 5), (70, 48, 64, 8), (300, 33, 41, 3), (3000, 72, 136, 64)])
+def test_slices_kept_elsewhere(dev, dtype, M, N, K, pad):
+    """x is a slice of a wider buffer, so the row stride of what comes back is another one."""
+    for i, act in enumerate(("none", "relu", "silu")):
+        for name in HOOKS:
+            t = make(M, N, K, dtype, dev, 7 * i + M, True, act != "relu", grad=False)
+            x = torch.cat((t["x"], torch.full((M, pad), float("nan"), device=dev, dtype=dtype)), 1)[:, :K]
+            assert x.stride(0) == K + pad
+            leaves = [v.requires_grad_(True) for v in (x, t["w"], t["bias"])]
+            drop, keep = drop_and_keep(M, N, 0.0 if act == "relu" else 0.3, dev)
+            with torch.autograd.graph.saved_tensors_hooks(*HOOKS[name]):
+                y = linear_act(*leaves, ACTS[act], t["res"], drop)
+            ref = formulas(x, t["w"], t["bias"], t["res"], act, keep, 0.3 if drop else 0, t["dy"])
+            check(y, ref["y"], f"{name} {act} y")
+            for k, got in zip(("dx", "dw", "dbias"), torch.autograd.grad(y, leaves, t["dy"])):
+                check(got, ref[k], f"{name} {act} {k}")
+
+
+@gpu
+@pytest.mark.parametrize("pin", [False, True])
+def test_offloaded_slice(dev, pin):
+    """torch's own offloading, by element and by channel."""
+    t = make(60, 24, 40, torch.bfloat16, dev, 3, True, False, grad=False)
+    x = torch.cat((t["x"], t["x"][:, :9]), 1)[:, :40].requires_grad_(True)
+    w = t["w"].requires_grad_(True)
+    drop, keep = drop_and_keep(60, 24, 0.5, dev, 20)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+        y = linear_act(x.view(3, 20, 40), w, t["bias"], LI.ACT_GELU, None, drop)
+    ref = formulas(x, w, t["bias"], None, "gelu", keep, 0.5, t["dy"])
+    for k, got in zip(("dx", "dw"), torch.autograd.grad(y, [x, w], t["dy"].view(3, 20, 24))):
+        check(got, ref[k], k)
+
+
+@gpu
+def test_another_tensor_is_refused(dev):
+    """Of another shape, type or device than the one that was kept."""
+    t = make(20, 16, 24, torch.float32, dev, 5)
+    drop = Drop(0.5, pair(1, 2, dev))
+    for give in (lambda v: v[:-1], lambda v: v.double(), lambda v: v.cpu(), lambda v: v.flatten().repeat(2)):
+        for f in (lambda: linear_act(t["x"], t["w"], t["bias"], LI.ACT_SILU, None, drop), lambda: dropout(t["x"], drop)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda v: v, give):
+                y = f()
+            with pytest.raises(RuntimeError, match="given back as"):
+                y.sum().backward()
