@@ -235,20 +235,21 @@ struct LinearActBackward : public torch::autograd::Node {
         const bool dx = task_should_compute_output(0), dw = task_should_compute_output(1),
                    db = task_should_compute_output(2);
         if (dx || dw || db) {
-            at::AutoDispatchBelowADInplaceOrView below;
-            const at::Tensor g = dy.contiguous();
-            const at::ScalarType type = g.scalar_type();
-            const c10::Device device = g.device();
-            const auto self = shared_from_this();
+            const at::ScalarType type = dy.scalar_type();
+            const c10::Device device = dy.device();
             c10::DeviceGuard guard(device);
-            int64_t ldx = m.K;
+            const auto self = shared_from_this();
             at::DimVector zshape = m.xshape;
             zshape.back() = m.N;
-            at::Tensor xs = unpacked(x, self, m.xshape, type, device, "linear_act: x");
-            if (xs.defined()) xs = as_rows(xs, ldx);
-            const at::Tensor ws = dense(unpacked(weight, self, {m.N, m.K}, type, device, "linear_act: weight")),
-                             zs = dense(unpacked(z, self, zshape, kept_type(type, m.act), device, "linear_act: z")),
-                             rs = dense(unpacked(rng, self, m.rshape, at::kLong, device, "linear_act: rng"));
+            // above autograd: a hook may run a checkpointed forward again, whose operators record their graphs
+            const at::Tensor xu = unpacked(x, self, m.xshape, type, device, "linear_act: x"),
+                             wu = unpacked(weight, self, {m.N, m.K}, type, device, "linear_act: weight"),
+                             zu = unpacked(z, self, zshape, kept_type(type, m.act), device, "linear_act: z"),
+                             ru = unpacked(rng, self, m.rshape, at::kLong, device, "linear_act: rng");
+            at::AutoDispatchBelowADInplaceOrView below;
+            int64_t ldx = m.K;
+            const at::Tensor g = dy.contiguous(), xs = xu.defined() ? as_rows(xu, ldx) : xu, ws = dense(wu), zs = dense(zu),
+                             rs = dense(ru);
             if (dx) out[0] = at::empty(m.xshape, g.options());
             if (dw) out[1] = at::empty({m.N, m.K}, g.options());
             if (db) out[2] = at::empty({m.N}, g.options());

@@ -77,3 +77,23 @@ def test_another_tensor_is_refused(dev):
                 y = f()
             with pytest.raises(RuntimeError, match="given back as"):
                 y.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("early_stop", [False, True])
+@pytest.mark.parametrize("last", ["linear_act", "dropout"])
+def test_checkpointed_behind_other_operators(dev, last, early_stop):
+    """The forward that a backward runs again records other operators' graphs, whichever of these nodes asks for it first."""
+    from torch.utils.checkpoint import checkpoint, set_checkpoint_early_stop
+    t = make(30, 24, 40, torch.float32, dev, 6, True, True)
+    drop = Drop(0.4, pair(6, 7, dev))
+    leaves = [t[k] for k in ("x", "w", "bias", "res")]
+
+    def block(x, w, b, r):
+        y = linear_act(torch.tanh(x) * torch.sigmoid(x), w, b, LI.ACT_SILU, r.exp())
+        return dropout(y * y, drop, r) if last == "dropout" else linear_act(y.sin(), w @ w.t(), b, LI.ACT_ELU, r, drop)
+
+    want = torch.autograd.grad(block(*leaves), leaves, t["dy"])
+    with set_checkpoint_early_stop(early_stop):
+        again = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, t["dy"])
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
