@@ -21,6 +21,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from ... import _hip
 from ...utils.horovod import rank
@@ -61,6 +62,39 @@ _HERE = nullcontext()
 def on_device(device):
     """Launches go to the current device: make it this one."""
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+class _Recorded(torch.autograd.Function):
+    """fn(*args) as a Python operator, which torch.jit.trace records as a call of it."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        with torch.enable_grad():
+            inner = [a.detach().requires_grad_(a.requires_grad) if torch.is_tensor(a) else a for a in args]
+            y = fn(*inner)
+        ctx.inner = inner, y
+        return y.detach()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        inner, y = ctx.inner
+        leaves = [k for k, a in enumerate(inner) if torch.is_tensor(a) and a.requires_grad]
+        grads = dict(zip(leaves, torch.autograd.grad(y, [inner[k] for k in leaves], dy, retain_graph=True)))
+        return (None, *(grads.get(k) for k in range(len(inner))))
+
+
+def run(fn, *args):
+    """fn(*args), for an fn that allocates its result and fills it by address: a trace would hold the allocation alone."""
+    return fn(*args) if torch._C._get_tracing_state() is None else _Recorded.apply(fn, *args)
+
+
+def rng_next(state, add):
+    used = torch.empty_like(state)
+    with on_device(state.device):
+        _hip.check(_hip.lib().psfm_rng_next(state.data_ptr(), add, used.data_ptr(), _hip.stream(state.device)),
+                   "psfm_rng_next")
+    return used
 
 
 def keep_mask(rows, cols, p, rng):
@@ -111,7 +145,7 @@ def dropout(x, drop, residual=None):
         wide = torch.promote_types(x.dtype, torch.float32)
         y = plain_drop(x.to(wide), drop)
         return (y if residual is None else y + residual.to(wide)).to(x.dtype)
-    return _hip.ext().dropout(x, residual, drop.p, drop.rng, drop.channels)
+    return run(_hip.ext().dropout, x, residual, drop.p, drop.rng, drop.channels)
 
 
 def dropout2d(x, drop, residual=None):
@@ -148,13 +182,10 @@ class CounterDropout(nn.Module):
             return None
         state = self.state
         if not state.is_cuda:
-            seed, offset = state.tolist()
-            state[1] = _int64(offset + 1)
-            return Drop(self.p, torch.tensor([_int64(seed + rank()), offset]), self.channels)
-        used = torch.empty_like(state)
-        with on_device(state.device):
-            _hip.check(_hip.lib().psfm_rng_next(state.data_ptr(), rank(), used.data_ptr(), _hip.stream(state.device)),
-                       "psfm_rng_next")
+            used = torch.stack((state[0] + rank(), state[1]))
+            state[1] += 1
+        else:
+            used = run(rng_next, state, rank())
         return Drop(self.p, used, self.channels)
 
     def forward(self, x, residual=None):

@@ -15,7 +15,7 @@ import torch
 import torch.nn.functional as F
 
 from ... import _hip
-from .dropout import check_drop, check_like, plain_drop
+from .dropout import check_drop, check_like, plain_drop, run
 from .fused import ACT_ELU, ACT_NONE, ACT_RELU, ACT_SIGMOID
 
 ACT_SILU, ACT_GELU = 4, 5   # PSFM_ACT_SILU, PSFM_ACT_GELU
@@ -50,7 +50,7 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):
             y = plain_drop(y, drop)
         return (y if residual is None else y + residual.to(wide)).to(x.dtype)
     p, rng, channels = (0.0, None, False) if drop is None else drop
-    return _hip.ext().linear_act(x, weight, bias, act, residual, p, rng, channels)
+    return run(_hip.ext().linear_act, x, weight, bias, act, residual, p, rng, channels)
 
 
 def conv1x1_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):
