@@ -90,7 +90,9 @@ __device__ __forceinline__ void times_slope(int act, const float (&z)[N], float 
     _Pragma("unroll") for (int k = 0; k < N; ++k) d[k] *= F; \
     break;
     switch (act) {
-        case PSFM_ACT_RELU: PSFM_EACH((z[k] > 0.0f ? 1.0f : 0.0f))
+        case PSFM_ACT_RELU:   // a selection: an infinite gradient of a value below 0 is none, and NaN passes its own
+            _Pragma("unroll") for (int k = 0; k < N; ++k) d[k] = z[k] <= 0.0f ? 0.0f : d[k];
+            break;
         case PSFM_ACT_SIGMOID: PSFM_EACH(slope_sigmoid(z[k]))
         case PSFM_ACT_ELU: PSFM_EACH((z[k] > 0.0f ? 1.0f : __expf(z[k])))
         case PSFM_ACT_SILU: PSFM_EACH(slope_silu(z[k]))
