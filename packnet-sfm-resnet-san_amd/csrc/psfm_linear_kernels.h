@@ -74,9 +74,10 @@ __device__ __forceinline__ float slope_silu(float z) {
     const float s = sigmoidf(z);
     return s * (1.0f + z * (1.0f - s));
 }
+// of exp(-|z|): 1 - s has lost both tails' scale
 __device__ __forceinline__ float slope_sigmoid(float z) {
-    const float s = sigmoidf(z);
-    return s * (1.0f - s);
+    const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return e * r * r;
 }
 template <typename T>
 __device__ __forceinline__ float slope_gelu(float z) {

@@ -53,3 +53,50 @@ def test_relu_selects_its_gradient(dev, dtype, M, N, K):
         ref = formulas(torch.zeros(1, K, device=dev, dtype=dtype), t["w"], None, None, "none", None, 0, passed)
         check(dx[3:4], (ref["dx"][0], ref["dx"][1] + 4 * U * (passed.abs() @ t["w"].detach().double().abs())), "row of a NaN")
         assert bool(db.isfinite().all()) and bool(dx.isfinite().all())
+
+
+def tails(act, z):
+    """act(z), act'(z) in float64 and the sums of magnitudes that their fp32 errors count from, with steps of 2^-24 each.
+    exp(a) of an fp32 a: a's own rounding and log2(e)'s are 2 |a| steps, the function, sums, reciprocals and products
+    after it 12 at most."""
+    steps = 2 * z.abs() + 12
+    s = torch.sigmoid(z)
+    t = torch.sigmoid(-z)
+    if act == "sigmoid":
+        return s, s * t, steps * U * s, steps * U * s * t
+    if act == "silu":
+        return z * s, s * (1 + z * t), steps * U * (z * s).abs(), steps * U * s * (1 + z.abs())
+    a, slope = torch.where(z > 0, z, torch.expm1(z)), torch.where(z > 0, 1.0, torch.exp(z))
+    return a, slope, steps * U * a.abs(), steps * U * slope
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["sigmoid", "elu", "silu"])
+def test_tails_keep_their_scale(dev, dtype, act):
+    """Relative bounds where the activations and their slopes are small: one rounding of the type, the steps of `tails`, and the
+    smallest values of the type (the hardware's exponential gives 0 below the normal ones)."""
+    f = torch.finfo(dtype)
+    v = torch.linspace(-13, 25, 4001, device=dev, dtype=torch.float64).to(dtype)
+    small = max(f.tiny * f.eps, 2.0 ** -125)
+
+    def near(got, value, err, what):
+        got, tol = got.detach().double().flatten(), f.eps / 2 * 1.02 * value.abs() + err + small
+        bad = (got - value).abs() / tol
+        assert bool((bad <= 1).all()), f"{what}: {float(bad.max())} of the bound at z = {float(v[int(bad.argmax())])}"
+
+    a, slope, ea, es = tails(act, v.double())
+    # z = x, one column; z = bias, few rows (no tiles) and more
+    x, w = v[:, None].clone().requires_grad_(True), torch.ones(1, 1, device=dev, dtype=dtype)
+    y = linear_act(x, w, None, ACTS[act])
+    near(y, a, ea, "y of x")
+    near(torch.autograd.grad(y, x, torch.ones_like(y))[0], slope, es, "dx")
+    for M, K in ((1, 8), (8, 8), (40, 8), (300, 64)):
+        x, w = torch.zeros(M, K, device=dev, dtype=dtype), torch.zeros(4001, K, device=dev, dtype=dtype, requires_grad=True)
+        b = v.clone().requires_grad_(True)
+        y = linear_act(x, w, b, ACTS[act])
+        dy = torch.zeros_like(y)
+        dy[M // 2] = 1
+        near(y[M - 1], a, ea, f"y of the bias, {M} rows")
+        near(torch.autograd.grad(y, b, dy, retain_graph=True)[0], slope, es, "dbias alone")
+        near(torch.autograd.grad(y, [b, w], dy)[0], slope, es, "dbias beside dw")
