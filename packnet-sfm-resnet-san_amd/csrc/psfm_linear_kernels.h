@@ -34,17 +34,18 @@ constexpr int CHUNK = 16 / (int)sizeof(T);   // values of one 16-byte chunk
 // v_rcp_f32 is good to one step of fp32, the IEEE division around it costs ten instructions
 __device__ __forceinline__ float sigmoidf(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-// The normal distribution function and exp(-z^2 / 2).  fp32: erff.  16 bits: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2),
-// t = 1 / (1 + p x), x >= 0 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: 1.5e-7 of error), which
-// shares its exponential with the density and keeps the lower tail's own scale.
+// The normal distribution function and exp(-z^2 / 2).  Both branches keep the lower tail's own scale.  fp32: erfcf.  16 bits,
+// sharing the density's exponential: erfc(x) = (a1 t + .. + a8 t^8) exp(-x^2), t = 1 / (1 + 0.44 x), x = |z| / sqrt(2).
+// The a are a fit of least relative error over x = 0 .. 10 (linear programming; 1 at x = 0): 1.8e-7, 5.7e-7 in fp32.
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     e = __expf(-0.5f * z * z);
     if constexpr (sizeof(T) == 4) {
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+        return 0.5f * erfcf(-0.70710678118654752f * z);
     } else {
-        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678118654752f * fabsf(z));
-        const float q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.44f * 0.70710678118654752f * fabsf(z));
+        const float a = t * (0.294311702f + t * (-0.276345044f + t * 0.0707828626f));
+        const float q = t * (0.248222306f + t * (0.24884516f + t * (0.217515379f + t * (0.214997917f + t * (-0.0183302537f + a)))));
         const float low = 0.5f * q * e;
         return z < 0.0f ? low : 1.0f - low;
     }

@@ -58,8 +58,13 @@ def test_relu_selects_its_gradient(dev, dtype, M, N, K):
 def tails(act, z):
     """act(z), act'(z) in float64 and the sums of magnitudes that their fp32 errors count from, with steps of 2^-24 each.
     exp(a) of an fp32 a: a's own rounding and log2(e)'s are 2 |a| steps, the function, sums, reciprocals and products
-    after it 12 at most."""
-    steps = 2 * z.abs() + 12
+    after it 12 at most.  The normal distribution's z^2 / 2, or z / sqrt(2) in erfc, whose logarithm has the slope
+    z^2 + 1 in it: 2 z^2 + 2, and 38 for erfc itself (16 units) and the rest."""
+    steps = 2 * z * z + 40 if act == "gelu" else 2 * z.abs() + 12
+    if act == "gelu":
+        c = torch.erfc(-z / math.sqrt(2)) / 2
+        d = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return z * c, c + d, steps * U * (z * c).abs(), steps * U * (c + d.abs())
     s = torch.sigmoid(z)
     t = torch.sigmoid(-z)
     if act == "sigmoid":
@@ -72,7 +77,7 @@ def tails(act, z):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("act", ["sigmoid", "elu", "silu"])
+@pytest.mark.parametrize("act", ["sigmoid", "elu", "silu", "gelu"])
 def test_tails_keep_their_scale(dev, dtype, act):
     """Relative bounds where the activations and their slopes are small: one rounding of the type, the steps of `tails`, and the
     smallest values of the type (the hardware's exponential gives 0 below the normal ones)."""
