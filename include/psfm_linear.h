@@ -35,7 +35,9 @@ extern "C" {
 #define PSFM_ACT_GELU 5    /* z (1 + erf(z / sqrt(2))) / 2  */
 
 typedef struct psfm_linear {
-    int64_t M, N, K;       /* any sizes >= 0; K = 0 is an empty sum                            */
+    int64_t M, N, K;       /* sizes >= 0; K = 0 is an empty sum.  What one launch does not hold returns -8: over
+                              2^31 - 256 rows of a few columns or columns of a few rows, over 2.5 10^8 columns
+                              where db is wanted                                              */
     int64_t ldx, ldr;      /* row strides of x and res in values (W, y, z, dy, dx, dw are dense) */
     int32_t dtype, act;
     double p;              /* dropout probability, 0: none                                     */

@@ -97,7 +97,7 @@ template <typename T>
 int run(const Args& a, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T), PER = THREADS * UNROLL;
     const int64_t blocks = (a.rows * ((a.cols + V - 1) / V) + PER - 1) / PER;
-    if (blocks > 0x7fffffff) return fail(-1, "psfm_dropout: more values than a launch holds");
+    if (blocks > 0xffffffffll / THREADS) return fail(-1, "psfm_dropout: more values than a launch holds");
     const dim3 grid((unsigned)blocks);
     if (a.drop.rng && a.drop.mask_rows > 1)
         a.res ? k_dropout<T, true, true><<<grid, THREADS, 0, s>>>(a) : k_dropout<T, false, true><<<grid, THREADS, 0, s>>>(a);

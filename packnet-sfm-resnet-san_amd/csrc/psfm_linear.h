@@ -94,14 +94,16 @@ const LinearOps& linear_ops_f16();
 const LinearOps& linear_ops_bf16();
 
 struct Tile {
-    int bi, bj;
+    int bi, bj, threads;
 };
-constexpr Tile LINEAR_TILES[] = {{64, 64}, {128, 128}, {256, 256}};
+constexpr Tile LINEAR_TILES[] = {{64, 64, 256}, {128, 128, 256}, {256, 256, 512}};
 constexpr int LINEAR_NTILES = 3;   // 32-bit types: the first two
-constexpr int DZ_THREADS = 256;
+constexpr int DZ_THREADS = 256, SKINNY_THREADS = 512, FINISH_THREADS = 256;
 // Chunks of columns in a k_dz workgroup: all of a narrow layer's, 32 of a wide one's (184320 x 64 bf16: 15.1 us with 8, 32.8
 // with 32; 100000 x 8: 11.0, 20.0; 4096 x 24: 6.1, 6.3).
 constexpr int DZ_NARROW = 8, DZ_WIDE = 32;
 constexpr int SKINNY_ROWS = 32;    // at most
+// Workgroups of one launch: the runtime counts a dimension's threads in 32 bits
+constexpr int64_t most_blocks(int threads) { return 0xffffffffll / threads; }
 
 }  // namespace psfm

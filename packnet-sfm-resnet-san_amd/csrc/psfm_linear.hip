@@ -57,6 +57,7 @@ struct Plan {
     int splits;
     double alone, busy, join;   // estimates: the larger of the first two, and the join
     int64_t blocks() const { return ti * tj * splits; }
+    bool fits() const { return blocks() <= most_blocks(LINEAR_TILES[variant].threads); }
 };
 
 // The tile and the splits of the reduction that should take least time, from what a stage of 128 bytes of reduction
@@ -96,6 +97,7 @@ Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, bool forward, i
         for (const int want : SPLITS) {
             const int64_t per = std::max<int64_t>(1, up(stages, want)), n = std::max<int64_t>(1, up(stages, per));
             if (want > 1 && (per < 2 || ti * tj * n > 4096)) break;
+            if (ti * tj * n > most_blocks(LINEAR_TILES[v].threads)) break;
             const double blocks = (double)ti * (double)tj * (double)n, load = staged ? 1.0 : std::min(1.0, blocks / 512);
             const double rounds = (double)up((int64_t)std::min(blocks, 1e15), 256), out = forward && n == 1 ? times[v].out : 0.0;
             const double alone = (double)per * times[v].alone * wait * (0.64 + 0.36 * load) + out;
@@ -105,6 +107,10 @@ Plan plan(const psfm_linear* d, int64_t I, int64_t J, int64_t R, bool forward, i
             const double t = std::max(alone, busy) + join;
             if (best.rsplit == 0 || t < least) least = t, best = Plan{v, ti, tj, per * stage, (int)n, alone, busy, join};
         }
+    }
+    if (best.rsplit == 0) {   // no launch holds it: the caller finds that it does not fit
+        const int v = staged ? 0 : std::min(largest, wide ? 1 : 2);
+        best = Plan{v, up(I, LINEAR_TILES[v].bi), up(J, LINEAR_TILES[v].bj), std::max<int64_t>(1, stages) * stage, 1, 1e30, 1e30, 0};
     }
     return best;
 }
@@ -118,7 +124,9 @@ bool mult(const void* p, int64_t ld, int64_t edge, int64_t v) {
 // Rows that one matrix instruction takes, or two where W's rows are short.  4096 x 4096 bf16, 16 rows: 9.9 us, 10.2 in
 // tiles; 32 rows: 13.6, 11.2.  1024 x 1024, 32 rows: 5.1, 6.5.  fp32 4096 x 4096, 16 rows: 20.1, 27.0; 32 rows: 28.9,
 // 27.8; 512 x 512, 32 rows: 6.2, 7.9.
-bool skinny(const psfm_linear* d) { return d->M <= 16 || (d->M <= SKINNY_ROWS && d->K * size_of(d->dtype) < 4096); }
+bool skinny(const psfm_linear* d) {
+    return (d->M <= 16 || (d->M <= SKINNY_ROWS && d->K * size_of(d->dtype) < 4096)) && up(d->N, 16) <= most_blocks(SKINNY_THREADS);
+}
 
 struct DzPlan {
     int64_t gx, gy, rows;
@@ -220,13 +228,11 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
     const LinearEpi e{y, bias, res, d->ldr, z, d->act, 1.0f, drop_of(d)};
     const int64_t v = 16 / size_of(d->dtype);
     const bool vec = mult(x, d->ldx, d->K, v) && mult(w, d->K, d->K, v);
-    if (skinny(d)) {
-        if (up(d->N, 16) > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more columns than a launch holds");
+    if (skinny(d))
         return status(o.skinny(vec, SkinnyArgs{x, w, d->ldx, d->M, d->N, d->K, e}, s), "psfm_linear_fwd: launch");
-    }
     const Plan p = plan(d, d->M, d->N, d->K, true);
     if (p.splits > 1 && !ws) return fail(-10, "psfm_linear_fwd: no workspace");
-    if (p.blocks() > 0x7fffffff) return fail(-8, "psfm_linear_fwd: more tiles than a launch holds");
+    if (!p.fits()) return fail(-8, "psfm_linear_fwd: more tiles than a launch holds");
     GemmArgs a{};
     a.P = x, a.Q = w, a.ldp = d->ldx, a.ldq = d->K, a.I = d->M, a.J = d->N, a.R = d->K, a.e = e;
     set(a, p, ws);
@@ -254,9 +260,10 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
                      (!b.stage || d->act == PSFM_ACT_NONE || ((uintptr_t)z & 15) == 0) &&
                      (!b.dx || ((uintptr_t)w & 15) == 0) && (!b.dw || mult(x, d->ldx, d->K, v));
     if (!vec) retile(b.pdx, d->M, d->K), retile(b.pdw, d->N, d->K);
-    const int64_t most = 0x7fffffff;
-    if (b.cols.gx > most || (b.dx && b.pdx.blocks() > most / 2) || (b.dw && b.pdw.blocks() > most / 2))
-        return fail(-8, "psfm_linear_bwd: more tiles than a launch holds");
+    // k_finish: 16 columns of db a workgroup, and the joins, whose products have at most 4096 tiles (plan): under 2^19 each
+    if ((b.pass && b.cols.gx > most_blocks(DZ_THREADS)) || (b.dx && !b.pdx.fits()) || (b.dw && !b.pdw.fits()) ||
+        (db && up(d->N, 16) + (1 << 20) > most_blocks(FINISH_THREADS)))
+        return fail(-8, "psfm_linear_bwd: more tiles or columns than a launch holds");
     const hipStream_t s = (hipStream_t)stream;
     const LinearOps& o = ops_of(d->dtype);
     const DropArgs drop = drop_of(d);
@@ -282,7 +289,8 @@ int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const v
         if (db && !b.pass) (b.parts ? (void*&)a.dz.cols : a.dz.db) = b.parts ? (void*)cols : db;
         set(a, b.pdw, at + b.dwp_at);
     }
-    const bool one = b.dx && b.dw && b.pdx.variant == b.pdw.variant;
+    const bool one = b.dx && b.dw && b.pdx.variant == b.pdw.variant &&
+                     b.pdx.blocks() + b.pdw.blocks() <= most_blocks(LINEAR_TILES[b.pdx.variant].threads);
     for (int part = 0; part < (one ? 1 : 2); ++part) {
         pair.ndx = b.dx && part == 0 ? pair.dx.blocks() : 0;
         pair.ndw = b.dw && (one || part == 1) ? pair.dw.blocks() : 0;

@@ -842,7 +842,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_pair(const PairArgs A) {
 // y of 16 columns and up to 16 MT rows.  The 8 waves take turns in the reduction, 128 bytes of each row (two steps) a
 // turn; each reads 16 rows of W straight into the matrix instructions' operands, U steps in flight, and x's few rows
 // from the caches.
-constexpr int SKINNY_WAVES = 8;
+constexpr int SKINNY_WAVES = SKINNY_THREADS / 64;
 
 template <typename T, int MT, bool VEC>
 __global__ __launch_bounds__(64 * SKINNY_WAVES) void k_skinny(const SkinnyArgs A) {
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(256) void k_join(const GemmArgs A) {
 
 // The bias gradient's parts: 16 columns a workgroup, 16 threads a column.
 template <typename T>
-__global__ __launch_bounds__(256) void k_finish(const FinishArgs A) {
+__global__ __launch_bounds__(FINISH_THREADS) void k_finish(const FinishArgs A) {
     __shared__ f4 sums[256];
     if (blockIdx.x < A.ndx) {
         join_any<T, false>(A.dx, blockIdx.x, sums);
@@ -1036,6 +1036,7 @@ bool deep(const GemmArgs& a) {
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool DEEP>
 void launch_forward(bool vec, const GemmArgs& a, hipStream_t s) {
+    static_assert(64 * WI * WJ == LINEAR_TILES[BI == 64 ? 0 : BI == 128 ? 1 : 2].threads, "a launch's threads");
     if (vec)
         k_forward<T, BI, BJ, WI, WJ, true, DEEP><<<dim3(a.blocks()), 64 * WI * WJ, 0, s>>>(a);
     else
@@ -1100,7 +1101,7 @@ int finish_of(FinishArgs& a, hipStream_t s) {
     a.ndw = a.dw.splits > 1 ? (uint32_t)join_blocks(a.dw) : 0;
     a.ncol = a.db ? (uint32_t)((a.N + 15) / 16) : 0;
     if (a.ndx + a.ndw + a.ncol == 0) return 0;
-    k_finish<T><<<dim3(a.ndx + a.ndw + a.ncol), 256, 0, s>>>(a);
+    k_finish<T><<<dim3(a.ndx + a.ndw + a.ncol), FINISH_THREADS, 0, s>>>(a);
     return (int)hipGetLastError();
 }
 

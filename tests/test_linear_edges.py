@@ -105,3 +105,50 @@ def test_tails_keep_their_scale(dev, dtype, act):
         near(y[M - 1], a, ea, f"y of the bias, {M} rows")
         near(torch.autograd.grad(y, b, dy, retain_graph=True)[0], slope, es, "dbias alone")
         near(torch.autograd.grad(y, [b, w], dy)[0], slope, es, "dbias beside dw")
+
+
+def test_more_than_a_launch_holds_is_refused():
+    """A launch's threads are counted in 32 bits; the check comes before anything is launched."""
+    L, a = _hip.lib(), ctypes.c_void_p(4096)
+    good = dict(M=4, N=8, K=8, ldx=8, ldr=8, dtype=2, act=0, p=0.0, mask_rows=1, rng=None)
+    for dtype in (0, 1, 2):
+        for sizes in (dict(M=2 ** 31), dict(N=2 ** 31, ldr=2 ** 31), dict(M=2 ** 33, N=1), dict(M=2 ** 17, N=2 ** 32, ldr=2 ** 32)):
+            d = _hip.Linear(**{**good, **sizes, "dtype": dtype})
+            assert L.psfm_linear_fwd(ctypes.byref(d), a, a, None, None, a, None, a, None) == -8, sizes
+            assert b"launch" in L.psfm_linear_last_error()
+            for act in (LI.ACT_NONE, LI.ACT_SILU):
+                d.act = act
+                assert L.psfm_linear_bwd(ctypes.byref(d), a, a, a, a, a, a, None, a, None) == -8, sizes
+        d = _hip.Linear(**{**good, "N": 2 ** 28, "ldr": 2 ** 28, "dtype": dtype})
+        assert L.psfm_linear_bwd(ctypes.byref(d), a, a, a, None, a, a, a, a, None) == -8
+        assert L.psfm_dropout(a, 1, None, 0, dtype, 2 ** 34, 1, 1, 0.5, a, a, None) == -1
+
+
+@gpu
+def test_rows_and_columns_past_the_smaller_launches(dev):
+    """More columns than the few-row kernel's launch holds (2^27), more rows than the smallest tiles' (2^30)."""
+    N, K = 2 ** 27 + 5, 8
+    t = make(1, 300, K, torch.bfloat16, dev, 2, True)
+    w = torch.zeros(N, K, device=dev, dtype=torch.bfloat16)
+    b = torch.zeros(N, device=dev, dtype=torch.bfloat16)
+    w[-300:], b[-300:] = t["w"].detach(), t["bias"].detach()
+    with torch.no_grad():
+        y = linear_act(t["x"], w, b, LI.ACT_GELU)
+    ref = formulas(t["x"], t["w"], t["bias"], None, "gelu", None, 0, t["dy"])
+    check(y[:, -300:], ref["y"], "columns")
+    assert bool((y[:, :-300] == 0).all())
+    del w, b, y
+    M, N = 2 ** 30 + 77, 1
+    t = make(300, N, K, torch.bfloat16, dev, 4, True, grad=False)
+    x = torch.zeros(M, K, device=dev, dtype=torch.bfloat16)
+    x[-300:] = t["x"]
+    dy = torch.zeros(M, N, device=dev, dtype=torch.bfloat16)
+    dy[-300:] = t["dy"]
+    leaves = [x.requires_grad_(True), t["w"].requires_grad_(True)]
+    y = linear_act(*leaves, t["bias"], LI.ACT_SILU)
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    ref = formulas(t["x"], t["w"], t["bias"], None, "silu", None, 0, t["dy"])
+    check(y[-300:], ref["y"], "rows")
+    check(dx[-300:], ref["dx"], "dx")
+    assert bool((dx[:-300] == 0).all())
+    check(dw, ref["dw"], "dw")
