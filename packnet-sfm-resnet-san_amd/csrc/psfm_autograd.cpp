@@ -108,15 +108,21 @@ void refuse_foreign_capture() {
 
 // A captured backward accumulates into a leaf on the stream that the leaf's accumulator is bound to, and an accumulator
 // lives as long as any graph of its leaf does.  One left from eager work on the default stream cannot take part in a
-// capture (the process ends in capture_end), so the forward is refused.
-void refuse_bound_leaf(const at::Tensor& t) {
-    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-    const std::optional<c10::Stream> s = accumulator ? accumulator->stream() : std::nullopt;
+// capture (the process ends in capture_end), so the forward is refused; and so where the leaf is reached through views and
+// casts (conv1x1_act's weight, autocast's copies), one of which may itself be such a node.
+void refuse_bound(const std::optional<c10::Stream>& s) {
     TORCH_CHECK(!s || s->id() != 0,
                 "psfm: a HIP-graph capture is in progress and a graph from eager work on the default stream still holds one "
                 "of this call's leaves, whose gradient a captured backward would accumulate on that stream.  Free the "
                 "outputs of that work first (or run it on a side stream)");
+}
+void refuse_bound_leaf(const at::Tensor& t) {
+    if (!t.defined() || !t.requires_grad()) return;
+    if (t.is_leaf()) {
+        if (const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t)) refuse_bound(accumulator->stream());
+        return;
+    }
+    for (auto f = t.grad_fn(); f; f = f->num_outputs() == 1 ? f->next_edge(0).function : nullptr) refuse_bound(f->stream());
 }
 
 // ---- tensors -------------------------------------------------------------------------------------

@@ -1,12 +1,15 @@
 """What linear_act and dropout keep for their backward pass, given back by saved-tensor hooks: from the host, with other
-strides, as another tensor.  Gradients against the formulas in float64 (test_linear.formulas derives the tolerances)."""
+strides, as another tensor; and the leaves that graphs hold.  Gradients against the formulas in float64
+(test_linear.formulas derives the tolerances)."""
+import gc
+
 import pytest
 import torch
 
 import packnet_sfm_amd  # noqa: F401
 from packnet_sfm_amd.networks.layers import linear as LI
-from packnet_sfm_amd.networks.layers.dropout import Drop, dropout
-from packnet_sfm_amd.networks.layers.linear import linear_act
+from packnet_sfm_amd.networks.layers.dropout import Drop, dropout, dropout2d
+from packnet_sfm_amd.networks.layers.linear import conv1x1_act, linear_act
 from test_dropout import pair
 from test_linear import ACTS, TYPES, check, drop_and_keep, formulas, make
 
@@ -97,3 +100,51 @@ def test_checkpointed_behind_other_operators(dev, last, early_stop):
     with set_checkpoint_early_stop(early_stop):
         again = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, t["dy"])
     assert all(torch.equal(a, b) for a, b in zip(want, again))
+
+
+@gpu
+def test_capture_with_a_leaf_behind_views_and_casts_is_refused(dev):
+    """As a bare leaf is (test_linear.py): the weight of a 1x1 convolution, an autocast copy, a permuted image, a view made before the
+    capture.  Freed, the same calls are captured, and replay what the eager calls give."""
+    g = torch.Generator().manual_seed(4)
+    n = lambda *s: torch.randn(*s, generator=g).to(dev).requires_grad_(True)  # noqa: E731
+    img, w, rows, drop = n(2, 16, 4, 5), n(24, 16, 1, 1), n(24, 16), Drop(0.5, pair(1, 1, dev))
+    buf = torch.zeros(8, device=dev)
+
+    def cast(t):
+        with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+            return linear_act(t.detach(), rows)
+
+    calls = {"weight": (w, lambda: conv1x1_act(img.detach(), w)), "cast": (rows, lambda: cast(rows)),
+             "image": (img, lambda: conv1x1_act(img, w.detach())), "dropped": (img, lambda: dropout2d(img, drop))}
+    for name, (leaf, call) in calls.items():
+        held = leaf.exp()
+        torch.autograd.grad(held, leaf, torch.ones_like(held), retain_graph=True)
+        with pytest.raises(RuntimeError, match="still holds one of this call's leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                buf.add_(1)
+                call()
+        torch.cuda.synchronize()
+        del held
+    view = w.flatten(1)
+    with pytest.raises(RuntimeError, match="still holds one of this call's leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            buf.add_(1)
+            linear_act(rows.detach(), view)
+    torch.cuda.synchronize()
+    del view
+    gc.collect()
+    for name, (leaf, call) in calls.items():
+        y = call()
+        dy = torch.ones_like(y)
+        want, = torch.autograd.grad(y, leaf, dy)
+        del y
+        gc.collect()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(call(), leaf, dy)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
