@@ -113,15 +113,18 @@ def keep_mask(rows, cols, p, rng):
     return words >= int(p * 2.0 ** 32 + 0.5)
 
 
-def plain_drop(t, drop):
-    """dropout of t in plain torch operations."""
+def plain_drop(t, drop, act=None):
+    """dropout of act(t) in plain torch operations."""
     shape = t.shape
     if t.numel() == 0:
         return t
     share = mask_rows(shape, drop.channels)
-    keep = keep_mask(t.numel() // shape[-1] // share, shape[-1], drop.p, drop.rng)
+    keep = keep_mask(t.numel() // shape[-1] // share, shape[-1], drop.p, drop.rng).unsqueeze(1)
     scale = 1.0 / (1.0 - drop.p) if drop.p < 1.0 else 0.0
-    return torch.where(keep.unsqueeze(1), t.reshape(-1, share, shape[-1]) * scale, 0.0).view(shape)
+    t = t.reshape(-1, share, shape[-1])
+    if act is not None:   # of a finite value where it is dropped, so that the slope there is finite too
+        t = act(torch.where(keep, t, 0.0))
+    return torch.where(keep, t * scale, 0.0).view(shape)
 
 
 def check_like(t, name, shape, x):

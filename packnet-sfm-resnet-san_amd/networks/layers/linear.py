@@ -45,9 +45,8 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, drop=None):
         drop = check_drop(drop, x.device)
     if not x.is_cuda or x.dtype not in _hip.DTYPES:
         wide = torch.promote_types(x.dtype, torch.float32)
-        y = _PLAIN[act](F.linear(x.to(wide), weight.to(wide), None if bias is None else bias.to(wide)))
-        if drop is not None:
-            y = plain_drop(y, drop)
+        z = F.linear(x.to(wide), weight.to(wide), None if bias is None else bias.to(wide))
+        y = _PLAIN[act](z) if drop is None else plain_drop(z, drop, _PLAIN[act])
         return (y if residual is None else y + residual.to(wide)).to(x.dtype)
     p, rng, channels = (0.0, None, False) if drop is None else drop
     return run(_hip.ext().linear_act, x, weight, bias, act, residual, p, rng, channels)

@@ -152,3 +152,31 @@ def test_rows_and_columns_past_the_smaller_launches(dev):
     check(dx[-300:], ref["dx"], "dx")
     assert bool((dx[:-300] == 0).all())
     check(dw, ref["dw"], "dw")
+
+
+@pytest.mark.parametrize("where", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_dropped_value_has_no_gradient_whatever_it_was(where):
+    """z infinite or NaN, dy infinite or NaN, at dropped places only: y and every gradient are those of zeros there."""
+    if where == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a ROCm GPU")
+    M, N, K = 12, 20, 9
+    drop, keep = drop_and_keep(M, N, 0.5, where)
+    t = make(M, N, K, torch.float32, torch.device(where), 3, False, False, grad=False)
+    # z is not finite in the columns that row 2 drops; rows 0 and 1, which keep some of them, are not looked at
+    off = (~keep[2]).nonzero().flatten()
+    for act in ACTS.values():
+        for bad in (float("inf"), -float("inf"), float("nan")):
+            bias = torch.zeros(N, device=where)
+            bias[off] = bad
+            x = t["x"][2:3]
+            grads = []
+            for b, dyv in ((bias, bad), (torch.zeros_like(bias), 0.0)):
+                b = b.requires_grad_(True)
+                xs = torch.cat((t["x"][:2], x)).requires_grad_(True)
+                y = linear_act(xs, t["w"], b, act, None, drop)
+                dy = torch.zeros_like(y)
+                dy[2] = torch.where(keep[2], t["dy"][2], torch.full((), dyv, device=where))
+                dx, = torch.autograd.grad(y, xs, dy)
+                grads.append((y[2], dx[2]))
+            for a, b in zip(*grads):
+                assert torch.equal(a, b) and bool(a.isfinite().all())
