@@ -163,8 +163,10 @@ def dropout2d(x, drop, residual=None):
 class CounterDropout(nn.Module):
     """Dropout whose masks are (seed, offset), the offset counted on the device: in training every forward draws
     the next one, also in a captured graph's replays.  The ranks of a data-parallel job, which hold the same
-    buffers, take seed + rank; the layers of one network take different first offsets.  The state is no part
-    of the state_dict: checkpoints of networks with nn.Dropout load as they are.
+    buffers, take seed + rank (jobs whose masks must differ take seeds further apart than their ranks); the layers of
+    one network take different first offsets.  The state is no part of the state_dict: checkpoints of networks with
+    nn.Dropout load as they are.  dropout_states(network) saves the layers' states beside it, and
+    load_dropout_states goes on from them; DDPTrainer.checkpoint() holds them under 'dropout'.
 
     A forward that is run again for its backward (activation checkpointing) would draw another mask: draw() before
     it, and give the Drop to dropout or linear_act inside."""
@@ -193,6 +195,21 @@ class CounterDropout(nn.Module):
 
     def forward(self, x, residual=None):
         return (dropout2d if x.dim() == 4 else dropout)(x, self.draw(), residual)
+
+
+def dropout_states(network):
+    """{module name: [seed, offset]} of the network's CounterDropout layers."""
+    return {n: m.state.tolist() for n, m in network.named_modules() if isinstance(m, CounterDropout)}
+
+
+@torch.no_grad()
+def load_dropout_states(network, states):
+    """Goes on from dropout_states' masks, in place: captured graphs hold the states' addresses."""
+    layers = {n: m for n, m in network.named_modules() if isinstance(m, CounterDropout)}
+    if set(layers) != set(states):
+        raise RuntimeError(f"dropout states of other layers: {sorted(set(layers) ^ set(states))}")
+    for n, m in layers.items():
+        m.state.copy_(torch.tensor(states[n], dtype=torch.int64))
 
 
 def _int64(v):

@@ -34,6 +34,7 @@ import torch
 import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel as DDP
 
+from ..networks.layers.dropout import dropout_states
 from ..utils import horovod as hvd
 
 
@@ -371,11 +372,15 @@ class DDPTrainer:
         load_network(net, ckpt['state_dict'], 'depth_net') strips the prefix as for a reference
         checkpoint.  Written with torch.save(), it loads with weights_only=True when `config` is None
         or a plain dict / list / scalar tree (a yacs CfgNode or another object would need the
-        unpickling loader; pass config as a dict)."""
+        unpickling loader; pass config as a dict).  A network with counter-based dropout has its masks' states
+        under 'dropout' (networks/layers/dropout.py load_dropout_states takes them), so that a resumed run
+        draws the masks that the run would have drawn."""
         sd = {"model." + k: v.detach().cpu() for k, v in self.state_dict().items()}
+        states = dropout_states(self.model)
         return {"config": config, "epoch": int(epoch), "state_dict": sd,
                 "optimizer": self.optimizer.state_dict(),
-                "scheduler": scheduler.state_dict() if scheduler is not None else None}
+                "scheduler": scheduler.state_dict() if scheduler is not None else None,
+                **({"dropout": states} if states else {})}
 
     def _zero_grad(self):
         """Model grads -> None (autograd then owns fresh, graph-static tensors); the fp32 master
