@@ -12,7 +12,7 @@ from packnet_sfm_amd.networks.layers import linear as LI
 from packnet_sfm_amd.networks.layers.dropout import Drop, dropout
 from packnet_sfm_amd.networks.layers.linear import conv1x1_act, linear_act
 from test_dropout import oracle_mask, pair
-from test_linear import ACTS, TYPES, U, check, drop_and_keep, formulas, make
+from test_linear import ACTS, CURVE, TYPES, U, check, drop_and_keep, formulas, make
 
 gpu = pytest.mark.gpu
 # rows x columns x reduction: gradients that make dz as they stage it, the same with odd rows, dz as a pass of its own
@@ -107,6 +107,26 @@ def test_tails_keep_their_scale(dev, dtype, act):
         near(torch.autograd.grad(y, [b, w], dy)[0], slope, es, "dbias beside dw")
 
 
+@gpu
+@pytest.mark.parametrize("act", ["sigmoid", "elu", "silu", "gelu"])
+@pytest.mark.parametrize("dtype,kept", [(torch.float32, 0.0), (torch.float16, 0.0), (torch.bfloat16, 2.0 ** -11)])
+def test_what_z_is_kept_in(dev, dtype, kept, act):
+    """Slopes at values of z between those of the layer's type: fp32 and fp16 layers keep z in fp32, bf16 ones in fp16, off by 2^-11 of
+    it, which moves the slope by at most |act''| times that.  Beside it the bounds of test_tails_keep_their_scale, and
+    two steps for z's own sum."""
+    f = torch.finfo(dtype)
+    b = torch.linspace(-6, 6, 4001, device=dev, dtype=torch.float64).to(dtype).requires_grad_(True)
+    x = torch.full((1, 1), 1.25 * 2.0 ** -9, device=dev, dtype=dtype)
+    w = torch.ones(4001, 1, device=dev, dtype=dtype, requires_grad=True)
+    z = b.detach().double() + float(x)
+    _, slope, _, es = tails(act, z)
+    tol = f.eps / 2 * 1.02 * slope.abs() + es + CURVE[act] * (kept + 2 * U) * z.abs() + f.tiny * f.eps
+    for some in ([b], [b, w]):
+        y = linear_act(x, w, b, ACTS[act])
+        got = torch.autograd.grad(y, some, torch.ones_like(y))[0].double()
+        assert bool(((got - slope).abs() <= tol).all()), float(((got - slope).abs() / tol).max())
+
+
 def test_more_than_a_launch_holds_is_refused():
     """A launch's threads are counted in 32 bits; the check comes before anything is launched."""
     L, a = _hip.lib(), ctypes.c_void_p(4096)
@@ -180,3 +200,48 @@ def test_a_dropped_value_has_no_gradient_whatever_it_was(where):
                 grads.append((y[2], dx[2]))
             for a, b in zip(*grads):
                 assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_gradients_that_are_dropped_reach_nothing(dev, dtype, M, N, K):
+    """dy infinite or NaN at dropped places: dx, dw and db, asked for together and each alone, are those of zeros there, whether
+    the products make dz as they stage it (dw's with the column sums) or a pass does."""
+    for act in ACTS.values():
+        t = make(M, N, K, dtype, dev, N, True, False)
+        drop, keep = drop_and_keep(M, N, 0.4, dev)
+        leaves = [t["x"], t["w"], t["bias"]]
+        y = linear_act(*leaves, act, None, drop)
+        zero = t["dy"].masked_fill(~keep, 0)
+        for bad in (float("inf"), float("nan")):
+            for some in (leaves, leaves[1:], leaves[:1], leaves[1:2], leaves[2:]):
+                a, b = (torch.autograd.grad(y, some, d, retain_graph=True) for d in (zero.masked_fill(~keep, bad), zero))
+                for u, v in zip(a, b):
+                    assert bool(u.isfinite().all()) and torch.equal(u, v)
+
+
+@gpu
+def test_counter_blocks_past_32_bits(dev):
+    """Masks of more than 2^34 values: the last rows' counters have a high word, in the dropout pass, in the product's epilogue
+    and in its gradients."""
+    rows = 2 ** 32 + 300
+    y = dropout(torch.ones(rows, 1, device=dev, dtype=torch.float16), Drop(0.25, pair(1, 2, dev)))
+    keep = torch.from_numpy(oracle_mask(600, 1, 0.25, 1, 2, rows - 600)).to(dev)
+    assert torch.equal(y[-600:] != 0, keep)
+    del y
+    M, N, K = 2 ** 20 + 64, 2 ** 14 + 8, 8
+    assert (M - 40) * (N // 4) > 2 ** 32
+    t = make(40, N, K, torch.bfloat16, dev, 4, True, grad=False)
+    x = torch.zeros(M, K, device=dev, dtype=torch.bfloat16)
+    x[-40:] = t["x"]
+    leaves = [x.requires_grad_(True), t["w"].requires_grad_(True)]
+    y = linear_act(*leaves, t["bias"], drop=Drop(0.25, pair(3, 2 ** 35, dev)))
+    keep = torch.from_numpy(oracle_mask(40, N, 0.25, 3, 2 ** 35, M - 40)).to(dev)
+    dy = torch.zeros(M, N, device=dev, dtype=torch.bfloat16)
+    dy[-40:] = t["dy"]
+    ref = formulas(t["x"], t["w"], t["bias"], None, "none", keep, 0.25, t["dy"])
+    check(y[-40:], ref["y"], "y")
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    check(dx[-40:], ref["dx"], "dx")
+    check(dw, ref["dw"], "dw")
