@@ -5,8 +5,7 @@
  *     y = res + drop(act(z))    res, y [M, N]
  *
  * a 1x1 convolution over the pixels of a channels_last activation (M = N*H*W rows of K channels: the
- * residual blocks' shortcut, packnet_sfm/networks/layers/packnet/layers01.py:40-61, and the pose
- * decoder's squeeze, packnet_sfm/networks/layers/resnet/pose_decoder.py:14-49), or a dense layer over
+ * residual blocks' shortcut, packnet_sfm/networks/layers/packnet/layers01.py:40-61), or a dense layer over
  * rows.  The mask of `drop` is psfm_dropout.h's over the [M, N] matrix: dropping y afterwards
  * with the same (seed, offset) is the same mask.
  *
@@ -56,7 +55,9 @@ int psfm_linear_fwd(const psfm_linear* d, const void* x, const void* w, const vo
 /* Workspace of the backward pass for the wanted gradients in bytes, or -1. */
 int64_t psfm_linear_bwd_ws_bytes(const psfm_linear* d, int want_dx, int want_dw, int want_db);
 /* With dz = drop(dy) act'(z):  dx = dz W [M, K], dw = dz^T x [N, K], db = sum over rows of dz [N]; each may
- * be NULL.  dy [M, N] dense.  z as the forward pass stored it (NULL for PSFM_ACT_NONE); for
+ * be NULL.  dz is fp32 where db sums it.  The products take it in the tensors' type: in 16 bits with an activation other than
+ * ReLU, small layers add a second product of what that rounding leaves (dx and dw are off by one rounding), the others
+ * do not (by up to 1.5 roundings).  In fp16 a dz, before dropout's scale, below 2^-25 is lost and one beyond 65504 is infinite.  dy [M, N] dense.  z as the forward pass stored it (NULL for PSFM_ACT_NONE); for
  * PSFM_ACT_RELU any tensor of its sign will do (y, where neither residual nor dropout touched it).
  * The gradient of res is dy itself. */
 int psfm_linear_bwd(const psfm_linear* d, const void* dy, const void* x, const void* w, const void* z, void* dx,

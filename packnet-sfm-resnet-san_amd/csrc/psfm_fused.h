@@ -11,9 +11,9 @@
 // One wave per (60-column stripe, RB-row band, image, scale).  The (at most two) contexts of a
 // target live in the two halves of 64-bit register pairs end to end: projection (pinhole: the
 // camera records of both contexts interleaved by the prepass, ws.cam_pairs, so every camera
-// entry is one SGPR pair operand of a v_pk_fma_f32), bilinear resolve, SSIM / L1, the SSIM
-// adjoint, the bilinear and projection adjoints and the dL/d[R|t] accumulation are v_pk_*
-// instructions for both contexts at once.  Lanes = columns c0-2..c0+61; the 60 inner lanes are
+// entry is one SGPR pair), bilinear resolve, SSIM / L1, the SSIM adjoint, the bilinear and
+// projection adjoints and the dL/d[R|t] accumulation are written for both contexts at once (two
+// scalar instructions each: the build keeps the compiler from packed fp32).  Lanes = columns c0-2..c0+61; the 60 inner lanes are
 // outputs (a 3x3 SSIM window of a 3x3 neighbourhood: halo 2).  Step k of the sweep:
 //   issue   row v = y0-2+k: target, sigmoid (prefetched one step earlier), lift/project and the
 //           12 bilinear gathers per context (results consumed at the END of the step, so their
@@ -213,7 +213,7 @@ typedef __attribute__((address_space(4))) const f2 cf2;
 // which halves the sampling positions' fp32 error against the lift + R X + t + K_ref chain
 // (max 1.4-1.8e-4 px vs 3.0-5.5e-4, mean 1.0e-5 vs 1.6e-5 over 1M KITTI-shaped points).  A lane's
 // column u is fixed for the whole sweep, so E's u- and constant columns are folded once per wave
-// (K12::ea) and a row costs e = ea + E[:, 1] v and two fma per entry of p: nine v_pk_fma for both
+// (K12::ea) and a row costs e = ea + E[:, 1] v and two fma per entry of p: nine pairs of fma for both
 // contexts, where the chain took 9 + 21.  The adjoint needs no intermediate point either:
 // dL/dd = dL/dp . dp/dd = dL/dp . (e + x).  dL/d[R|t] is accumulated as dL/dp (X, 1)^T and taken
 // through K_ref^T once per wave (bwd_pose_rows).

@@ -70,7 +70,7 @@ struct Plan {
 // 256 x 1024 x 4096: 11.1 in four pieces, 12.2 in two.  512 x 4096 x 4096: 26.9, 128 tiles in four pieces 31.3).  Rows that
 // are no whole chunks go through registers, and wait for memory half as long again.  STAGED: dz made on the way, whose
 // every stage waits for its loads and the activation's slope (8192 x 2048, reduction 128 in bf16: 41 us in 16 pieces, 42 in
-// 8, 220 in one).
+// 8, 220 in one).  It is one cost for all: measured with a slope and dz's rest, too high for ReLU and for none, which have neither.
 struct TileTime {
     double alone, busy, out;
 };
@@ -167,8 +167,9 @@ constexpr int64_t FEW_DZ = 1 << 15;
 // 8.3 with a pass; 480 x 64 x 64 9.5, 10.9; 480 x 512 x 256 13.8, 11.9; 184320 x 128 x 64 64, 51; 8192 x 256 x 2048 126, 52.
 // fp32: 480 x 64 x 256 10.2, 15.8; 30720 x 128 x 64 29, 35; 184320 x 256 x 64 195, 177; 8192 x 256 x 2048 242, 186.  A pass
 // rounds dz to the type once more, 16 bits off by up to sqrt(2) of one rounding where that averages over many values; with
-// few of them (1.49 was seen at 1500) the products make it for some microseconds more too.  The choice is the layer's, for all gradients together: what one of them is does not depend
-// on which others are asked for.
+// few of them (1.49 was seen at 1500) the products make it for some microseconds more too.  (fp16, either way: a dz below 2^-25 is lost, one
+// beyond 65504 infinite; no scale is safe for all of dy's range.)  The choice is the layer's, for all gradients together: what dx and dw are
+// does not depend on which others are asked for (db sums its rows in another order where no dw is made beside it).
 BwdPlan bwd_plan(const psfm_linear* d, bool want_dx, bool want_dw, bool want_db) {
     BwdPlan b{};
     const bool any = d->M > 0 && d->N > 0, make = d->act != PSFM_ACT_NONE || drop_of(d).rng;

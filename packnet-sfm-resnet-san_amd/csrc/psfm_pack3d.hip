@@ -43,7 +43,7 @@ int fail(int code, const std::string& msg) {
 }
 
 constexpr int NTH = 256;
-typedef float f2 __attribute__((ext_vector_type(2)));   // packed f32 pair (v_pk_fma_f32)
+typedef float f2 __attribute__((ext_vector_type(2)));   // f32 pair
 constexpr int P3D_WAVES = 2;
 #ifndef P3D_FWD_MFMA_DEFAULT
 #define P3D_FWD_MFMA_DEFAULT 0   // 1: the matrix-core forward for d = 4 pack layers too
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(P3D_WAVES))
 // consecutive k of a 4 x 16 pixel x 16 k chunk, both k in the halves of packed f32 pairs.  The
 // per-(pixel, o) run is stored from k0-1 (index 0) so that the four values (k-1, k, k+1, k+2) a
 // thread needs per pixel column are two aligned 8-byte LDS reads: (k-1, k) and (k+1, k+2) are the
-// dz = 2 and dz = 0 operand pairs, (k, k+1) the dz = 1 pair — 12 ds_read_b64 feed 36 v_pk_fma_f32
+// dz = 2 and dz = 0 operand pairs, (k, k+1) the dz = 1 pair — 12 ds_read_b64 feed 36 pairs of fma
 // (72 MACs) per (o, dy) where the one-k form spent 18 ds_read_b32 on 36 MACs.
 // One 16-k chunk per workgroup on an XCD-aware 1-D grid: a 128-byte line of a (pixel, o) dy run
 // holds 64 k = four chunks, and the four workgroups that read it run back to back on ONE XCD (the
@@ -603,8 +603,8 @@ __global__ __launch_bounds__(128, 2) void k_p3d_bwd_x_cl(P3 a, int gxn, int gyn)
                         const f2 c0 = dz == 0 ? pb[q + 2] : dz == 1 ? pm[q + 2] : pa[q + 2];
                         const f2 c1 = dz == 0 ? pb[q + 1] : dz == 1 ? pm[q + 1] : pa[q + 1];
                         const f2 c2 = dz == 0 ? pb[q] : dz == 1 ? pm[q] : pa[q];
-                        // one fused multiply-add chain per pair (3 v_pk_fma_f32; the sum-then-add
-                        // form took 4 packed ops per 3 MAC pairs)
+                        // one fused multiply-add chain per pair (the sum-then-add form takes 4
+                        // operations per 3 MACs)
                         acc[q] = w0 * c0 + acc[q];
                         acc[q] = w1 * c1 + acc[q];
                         acc[q] = w2 * c2 + acc[q];

@@ -184,8 +184,8 @@ __device__ __forceinline__ DepthChain depth_chain(const psfm_params& p) {
 
 // ---------------------------------------------------------------------------------------------
 // Packed candidate arithmetic (v3): the contexts of a target are evaluated in PAIRS, one
-// context per half of a 64-bit register pair, so every SSIM / L1 / blend operation is one
-// v_pk_{add,mul,fma}_f32 for two candidates.  Odd NC: the last pair's high half duplicates
+// context per half of a 64-bit register pair, so every SSIM / L1 / blend operation is written once
+// for two candidates (two scalar instructions: the build keeps the compiler from packed fp32).  Odd NC: the last pair's high half duplicates
 // the last context (computed, never read).
 // ---------------------------------------------------------------------------------------------
 typedef float f2 __attribute__((ext_vector_type(2)));

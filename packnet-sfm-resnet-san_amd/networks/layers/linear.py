@@ -6,10 +6,12 @@
                                                      channels_last storage is the product's rows
 
 The residual blocks' shortcut (packnet_sfm/networks/layers/packnet/layers01.py:40-61: 1x1 convolution, channel
-dropout, sum) and the pose decoder's squeeze (packnet_sfm/networks/layers/resnet/pose_decoder.py:14-49) are of this
-form.  fp32, fp16 and bf16 tensors on a ROCm device run the HIP kernels, forward and backward; under autocast the
-tensors are cast to its type first, as torch's linear does.  Anything else (CPU tensors, fp64) runs the same
-arithmetic as plain torch ops.  The autograd node is in C++ (csrc/psfm_autograd.cpp).
+dropout, sum) is of this form and runs on it with dropout_seed (layers01.ResidualConv).  fp32, fp16 and bf16 tensors on
+a ROCm device run the HIP kernels, forward and backward; under autocast the tensors are cast to its type first, as
+torch's linear does.  Anything else (CPU tensors, fp64) runs the same arithmetic as plain torch ops.  Gradients: z is
+kept in fp16 for bf16 layers and in fp32 for the others, and large 16-bit layers round dz to their type before its
+products (include/psfm_linear.h).  The autograd node is in C++ (csrc/psfm_autograd.cpp); under torch.jit.trace a call
+is recorded as a Python operator.
 """
 import torch
 import torch.nn.functional as F
