@@ -163,7 +163,7 @@ double together(const BwdPlan& b) {
 constexpr int64_t FEW_DZ = 1 << 15;
 
 // The products make dz themselves, in the smallest tiles, where that should take less time than a pass of its own, a launch
-// and dz's way to memory and back.  bf16, both gradients and the bias's (rows x K x N): 64 x 4096 x 64 5.2 us,
+// and dz's way to memory and back.  bf16, both gradients and the bias's, replayed in a graph (rows x K x N): 64 x 4096 x 64 5.2 us,
 // 8.3 with a pass; 480 x 64 x 64 9.5, 10.9; 480 x 512 x 256 13.8, 11.9; 184320 x 128 x 64 64, 51; 8192 x 256 x 2048 126, 52.
 // fp32: 480 x 64 x 256 10.2, 15.8; 30720 x 128 x 64 29, 35; 184320 x 256 x 64 195, 177; 8192 x 256 x 2048 242, 186.  A pass
 // rounds dz to the type once more, 16 bits off by up to sqrt(2) of one rounding where that averages over many values; with

@@ -64,6 +64,9 @@ def on_device(device):
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+_tracing = torch._C._get_tracing_state
+
+
 class _Recorded(torch.autograd.Function):
     """fn(*args) as a Python operator, which torch.jit.trace records as a call of it."""
 
@@ -86,7 +89,7 @@ class _Recorded(torch.autograd.Function):
 
 def run(fn, *args):
     """fn(*args), for an fn that allocates its result and fills it by address: a trace would hold the allocation alone."""
-    return fn(*args) if torch._C._get_tracing_state() is None else _Recorded.apply(fn, *args)
+    return fn(*args) if _tracing() is None else _Recorded.apply(fn, *args)
 
 
 def rng_next(state, add):
